@@ -41,7 +41,7 @@ SLTX_F32 = 2
 SLTX_EPI_NONE = 0
 SLTX_EPI_GELU_TANH = 2
 
-# Every symbol include/swiftltx_q4.h declares.
+# Every symbol the headers in include/ declare.
 EXPORTED = (
     "sltx_abi_version",
     "sltx_init",
@@ -75,6 +75,13 @@ EXPORTED = (
     "sltx_st_read_host",
     "sltx_st_read_device",
     "sltx_st_read_device_f32",
+    "sltx_attention",
+    "sltx_attention_cached",
+    "sltx_attention_cached_workspace",
+    "sltx_kv_append",
+    "sltx_kv_accept",
+    "sltx_kv_evict",
+    "sltx_kv_evict_workspace",
 )
 
 
@@ -105,6 +112,27 @@ class CSampleState(ctypes.Structure):
         ("next_draw", ctypes.c_void_p),
         ("draw_count", ctypes.c_int32),
     ]
+
+
+class CAttentionArgs(ctypes.Structure):
+    """sltx_attention_args."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v", "out")]
+                + [(n, ctypes.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "out_stride")]
+                + [(n, ctypes.c_int32) for n in ("dtype", "batch", "q_rows", "k_rows", "q_heads",
+                                                 "kv_heads", "head_dim", "causal")]
+                + [("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("bias", ctypes.c_void_p),
+                   ("bias_head_stride", ctypes.c_int64), ("bias_len", ctypes.c_int32),
+                   ("bias_zero", ctypes.c_int32)]
+                + [(n, ctypes.c_void_p) for n in ("prefix", "q_docs", "k_docs", "q_lens", "k_lens")])
+
+
+class CKVCache(ctypes.Structure):
+    """sltx_kv_cache."""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("k", "v", "weight", "position", "length",
+                                                "next_position")]
+                + [(n, ctypes.c_int32) for n in ("layers", "batch", "kv_heads", "capacity", "head_dim",
+                                                 "dtype")]
+                + [("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)])
 
 
 _lib = None
@@ -187,6 +215,20 @@ def lib():
         L.sltx_st_read_device.restype = ctypes.c_int
         L.sltx_st_read_device_f32.argtypes = [VP, ctypes.c_char_p, VP, U64, VP]
         L.sltx_st_read_device_f32.restype = ctypes.c_int
+        S = ctypes.POINTER(ctypes.c_int64)
+        C = ctypes.POINTER(CKVCache)
+        L.sltx_attention.argtypes = [ctypes.POINTER(CAttentionArgs), P]
+        L.sltx_attention_cached.argtypes = [P, S, C, I32, I32, I32, F, F, P, I32, P, P]
+        L.sltx_kv_append.argtypes = [P, S, P, S, P, S, C, I32, I32, I32, P, I32, I32, P, P, P]
+        L.sltx_kv_accept.argtypes = [C, I32, P, I32, P, P]
+        L.sltx_kv_evict.argtypes = [C, I32, I32, I32, P]
+        for n in ("sltx_attention", "sltx_attention_cached", "sltx_kv_append", "sltx_kv_accept",
+                  "sltx_kv_evict"):
+            getattr(L, n).restype = ctypes.c_int
+        L.sltx_attention_cached_workspace.argtypes = [C, I32, I32, I32]
+        L.sltx_attention_cached_workspace.restype = I64
+        L.sltx_kv_evict_workspace.argtypes = [C, I32]
+        L.sltx_kv_evict_workspace.restype = I64
         _lib = L
     return _lib
 
@@ -882,3 +924,7 @@ def load_safetensors(directory):
     file in the directory, sorted by file name."""
     names = sorted(f for f in os.listdir(directory) if f.endswith(".safetensors"))
     return [SafeTensorsFile(os.path.join(directory, f)) for f in names]
+
+
+from .attn import (KVCache, attention, attention_cached, distance_bias, kv_accept,  # noqa: E402
+                   kv_append, kv_evict, rope_inv_freq, tree_masks)

@@ -1,0 +1,358 @@
+// attn_few.hip -- attention of few query rows over a key/value cache (a decoded
+// token, a small tree of drafted tokens), the parts of split attentions joined,
+// and attention weights added up per key.
+//
+// At most 32 rows, those of all query heads that share a key/value head, against
+// thousands of keys: bound by reading the cache once.  A block takes one range
+// of the keys of one head; its four waves take 32 keys each at a time, every
+// wave with its own two stages of LDS, so nothing waits for another wave until
+// the waves' sums are added at the end.
+#include "attn_tile.hpp"
+
+namespace sltx {
+
+enum : int { kCap = 1, kSplit = 2 };
+constexpr int kWaveKeys = kFewKeys / 4;   // keys of a wave's tile
+
+template <int D, bool BF, int MODE>
+__global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnParams p) {
+    constexpr bool CAP = MODE & kCap, SPLIT = MODE & kSplit;
+    constexpr int TILE = kWaveKeys * D;      // values of a tile
+    constexpr int QT = D / 16, DB = D / 32;
+    constexpr int INSTR = TILE * 2 / 1024;   // copies of a tile
+    constexpr int PITCH = D + 4;             // of the waves' sums in LDS
+    constexpr int STAGES = 4 * 2 * 2 * TILE * 2, SUMS = 4 * kFewRows * PITCH * 4;
+    __shared__ __attribute__((aligned(1024))) char lds[STAGES > SUMS ? STAGES : SUMS];
+    __shared__ float mls[4][kFewRows][2];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, h = lane >> 5;
+    const int split = SPLIT ? blockIdx.x % p.splits : 0;
+    const int bh = SPLIT ? blockIdx.x / p.splits : blockIdx.x;
+    const int hb = bh % p.heads, b = bh / p.heads;
+    const SeqLens len = seq_lens(p, b);
+    const int rows = p.Sq * p.pack;
+
+    const bool has_row = n < rows;
+    const int qi = has_row ? n / p.pack : 0;
+    const int head = hb * p.pack + (has_row ? n % p.pack : 0);
+    const int units = (len.k + kFewKeys - 1) / kFewKeys;
+    int first = 0, last = units;
+    if (SPLIT) {
+        const int each = (units + p.splits - 1) / p.splits;
+        first = min(units, split * each);
+        last = min(units, first + each);
+    }
+    const int kstride = (int)p.ks.r * 2, vstride = (int)p.vs.r * 2, head_bytes = p.D * 2;
+    const uint16_t* kbase = p.k + b * p.ks.b + hb * p.ks.h;
+    const uint16_t* vbase = p.v + b * p.vs.b + hb * p.vs.h;
+    TileCopy<D, false, INSTR> kc;
+    TileCopy<D, true, INSTR> vc;
+    kc.init(0, lane, kstride, head_bytes);
+    vc.init(0, lane, vstride, head_bytes);
+    // this wave's stages: K, V, K, V
+    const uint32_t mine = lds_offset(lds) + wave * (4 * TILE * 2);
+    // the wave's tile of unit u; a tile past the last key is not copied
+    auto copy = [&](int u, int stage) {
+        const int j0 = u * kFewKeys + wave * kWaveKeys;
+        const int left = min(kWaveKeys, len.k - j0);
+        if (left <= 0) return;
+        const u32x4 kr = tile_rsrc(kbase + j0 * p.ks.r, left, kstride, head_bytes);
+        const u32x4 vr = tile_rsrc(vbase + j0 * p.vs.r, left, vstride, head_bytes);
+        const uint32_t at = mine + stage * (2 * TILE * 2);
+#pragma unroll
+        for (int i = 0; i < INSTR; ++i) copy_1k(kr, kc.off[i], at + i * 1024);
+#pragma unroll
+        for (int i = 0; i < INSTR; ++i) copy_1k(vr, vc.off[i], at + TILE * 2 + i * 1024);
+    };
+    if (first < last) copy(first, 0);
+    if (first + 1 < last) copy(first + 1, 1);
+
+    u32x4 qf[QT];
+    {
+        const uint16_t* q = p.q + b * p.qs.b + (int64_t)qi * p.qs.r + (int64_t)head * p.qs.h;
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            const int c = 16 * t + 8 * h;
+            qf[t] = has_row && c < p.D ? *reinterpret_cast<const u32x4*>(q + c) : u32x4{};
+        }
+    }
+    // the row sees the keys below lim, but for the tree
+    const int lim = p.tree ? len.k : min(len.k, len.old + qi + 1);
+    const uint64_t tree = p.tree && has_row ? p.tree[b * (int64_t)p.Sq + qi] : 0;
+    auto in_tree = [&](int j) { return j < len.old || (tree >> ((j - len.old) & 63) & 1); };
+
+    f32x16 o[DB];
+#pragma unroll
+    for (int i = 0; i < DB; ++i) o[i] = f32x16{};
+    RowState st = {-kInf, 0.0f, 0.0f};
+    const float f = CAP ? kLog2e : p.scale * kLog2e;
+    const float grow = 8.0f / f;
+    const float yscale = CAP ? p.scale / p.cap : 0.0f;
+    const uint32_t kfrag = k_frag_base<D>(lane), vfrag = v_frag_base<D>(lane);
+    int stage = 0;
+    for (int u = first; u < last; ++u, stage ^= 1) {
+        const int j0 = u * kFewKeys + wave * kWaveKeys;
+        if (j0 >= len.k) break;   // only in the last unit
+        // the next tile's copies may stay in flight
+        if (u + 1 < last && j0 + kFewKeys < len.k) copies_wait<2 * INSTR>();
+        else copies_wait<0>();
+        const uint32_t kt = mine + stage * (2 * TILE * 2), vt = kt + TILE * 2;
+        const bool all = j0 + kWaveKeys <= len.old;
+        uint32_t bad = 0;   // keys whose V rows are not finite
+        if (!all) {
+#pragma unroll
+            for (int i = 0; i < TILE / 8 / 64; ++i) {
+                constexpr int P = D / 8;
+                const uint64_t m = __ballot(clear_piece<BF>(vt + (i * 64 + lane) * 16));
+#pragma unroll
+                for (int k = 0; k < 64 / P; ++k)
+                    bad |= (m >> (k * P) & ((1u << P) - 1)) ? 1u << (i * (64 / P) + k) : 0;
+            }
+        }
+        f32x16 s = {};
+#pragma unroll
+        for (int t = 0; t < QT; ++t) s = mfma32<BF>(k_frag<D>(kt, kfrag, 0, t), qf[t], s);
+        if constexpr (CAP) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = capped(s[i] * yscale, p.cap);
+        }
+        if (!all) {
+            const int d = lim - j0 - 4 * h;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = 8 * (i / 4) + i % 4 < d ? s[i] : -kInf;
+            if (p.tree) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    s[i] = in_tree(j0 + 8 * (i / 4) + 4 * h + i % 4) ? s[i] : -kInf;
+            }
+        }
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+        top = half_max(top);
+        if (__any(top > st.m + grow)) {
+            const float m = fmaxf(st.m, top);
+            const float mf = m == -kInf ? 0.0f : m * f;
+            const float a = st.m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(st.mf - mf);
+            st.m = m;
+            st.mf = mf;
+            st.l *= a;
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[i][e] *= a;
+        }
+        u32x4 pf[2];
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const float w0 = __builtin_amdgcn_exp2f(s[i] * f - st.mf);
+            const float w1 = __builtin_amdgcn_exp2f(s[i + 1] * f - st.mf);
+            st.l += w0 + w1;
+            pf[i / 8][i % 8 / 2] = pack2<BF>(w0, w1);
+        }
+        weigh_values<D, BF, 2>(o, pf, vt, vfrag);
+        while (bad) {
+            const int j = j0 + __builtin_ctz(bad);
+            bad &= bad - 1;
+            const bool mine = has_row && j < lim && (!p.tree || in_tree(j));
+            add_values<D, BF>(o, vbase + j * p.vs.r, p.D, h, mine);
+        }
+        // the stage is free once every read of it has returned
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (u + 2 < last) copy(u + 2, stage);
+    }
+
+    // ---- the waves' sums ----
+    const float l = half_sum(st.l);
+    __syncthreads();   // no wave reads its stages any more
+    float* sums = reinterpret_cast<float*>(lds);
+    if (has_row) {
+        float* po = sums + (wave * kFewRows + n) * PITCH;
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f32x4*>(po + 32 * db + 8 * i + 4 * h) =
+                    f32x4{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
+        if (h == 0) mls[wave][n][0] = st.m == -kInf ? -kInf : st.mf, mls[wave][n][1] = l;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < rows * (D / 4); e += 256) {
+        const int r = e / (D / 4), c = e % (D / 4) * 4;
+        float m = -kInf;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) m = fmaxf(m, mls[w][r][0]);
+        f32x4 x = {};
+        float lsum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float a = mls[w][r][0] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(mls[w][r][0] - m);
+            lsum += a * mls[w][r][1];
+            // a wave without keys has sums of 0; a weight of 0 must not meet an infinity
+            const f32x4 y = *reinterpret_cast<const f32x4*>(sums + (w * kFewRows + r) * PITCH + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] += a == 0.0f ? 0.0f : a * y[i];
+        }
+        if constexpr (SPLIT) {
+            const int64_t at = ((int64_t)bh * p.splits + split) * rows + r;
+            *reinterpret_cast<f32x4*>(p.part_o + at * D + c) = x;
+            if (c == 0) *reinterpret_cast<f32x2*>(p.part_ml + at * 2) = f32x2{m, lsum};
+        } else if (c < p.D) {
+            const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+            uint16_t* out = p.out + b * p.os.b + (int64_t)(r / p.pack) * p.os.r +
+                            (int64_t)(hb * p.pack + r % p.pack) * p.os.h;
+            *reinterpret_cast<u32x2*>(out + c) =
+                u32x2{pack2<BF>(x[0] * inv, x[1] * inv), pack2<BF>(x[2] * inv, x[3] * inv)};
+        }
+    }
+}
+
+// One block for each row: out = sum over the splits of exp2(m_s - m) part_s,
+// divided by the same sum of their l.  Four waves take every fourth split.
+template <int D, bool BF>
+__global__ __launch_bounds__(256) void attn_combine_kernel(AttnParams p) {
+    constexpr int PER = D / 64;
+    __shared__ float sums[4][D];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rows = p.Sq * p.pack, row = blockIdx.x % rows, bh = blockIdx.x / rows;
+    const int hb = bh % p.heads, b = bh / p.heads;
+    const int64_t at = (int64_t)bh * p.splits * rows + row;   // of split 0
+    float m = -kInf;
+    for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, p.part_ml[(at + (int64_t)s * rows) * 2]);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    float l = 0.0f;
+    for (int s = lane; s < p.splits; s += 64) {
+        const f32x2 x = *reinterpret_cast<const f32x2*>(p.part_ml + (at + (int64_t)s * rows) * 2);
+        if (x[0] != -kInf) l += __builtin_amdgcn_exp2f(x[0] - m) * x[1];
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o, 64);
+    float x[PER] = {};
+#pragma unroll 4
+    for (int s = wave; s < p.splits; s += 4) {
+        const float ms = p.part_ml[(at + (int64_t)s * rows) * 2];
+        const float a = ms == -kInf ? 0.0f : __builtin_amdgcn_exp2f(ms - m);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            // a split without keys wrote no sums worth reading
+            const float y = p.part_o[(at + (int64_t)s * rows) * D + i * 64 + lane];
+            x[i] += a == 0.0f ? 0.0f : a * y;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) sums[wave][i * 64 + lane] = x[i];
+    __syncthreads();
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (p.row_ml && threadIdx.x == 0)
+        *reinterpret_cast<f32x2*>(p.row_ml + ((int64_t)bh * rows + row) * 2) = f32x2{m == -kInf ? 0.0f : m, inv};
+    const int c = threadIdx.x * 2;
+    if (c < p.D) {
+        const float y0 = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+        const float y1 = (sums[0][c + 1] + sums[1][c + 1]) + (sums[2][c + 1] + sums[3][c + 1]);
+        uint16_t* out = p.out + b * p.os.b + (int64_t)(row / p.pack) * p.os.r +
+                        (int64_t)(hb * p.pack + row % p.pack) * p.os.h;
+        *reinterpret_cast<uint32_t*>(out + c) = pack2<BF>(y0 * inv, y1 * inv);
+    }
+}
+
+// weight[key] += sum over rows r < wrows of exp2(f x_r - mf_r) / l_r.  S = Q K^T
+// this way round, so that a lane holds 16 rows of one key: the sum over rows is
+// its own.  A wave takes 32 keys; K's fragments come straight from memory.
+template <int D, bool BF, bool CAP>
+__global__ __launch_bounds__(256) void attn_weights_kernel(AttnParams p, float* weight, int wrows) {
+    constexpr int QT = D / 16;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n = lane & 31, h = lane >> 5;
+    const int bh = blockIdx.y, hb = bh % p.heads, b = bh / p.heads;
+    const SeqLens len = seq_lens(p, b);
+    const int rows = p.Sq * p.pack;
+    const float f = CAP ? kLog2e : p.scale * kLog2e;
+    const float yscale = CAP ? p.scale / p.cap : 0.0f;
+    const float* row_ml = p.row_ml + (int64_t)bh * rows * 2;
+    for (int j0 = (blockIdx.x * 4 + wave) * 32; j0 < len.k; j0 += gridDim.x * 128) {
+        const int j = j0 + n, jc = min(j, len.k - 1);
+        const uint16_t* k = p.k + b * p.ks.b + hb * p.ks.h + jc * p.ks.r;
+        u32x4 kf[QT];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            const int c = 16 * t + 8 * h;
+            kf[t] = c < p.D ? *reinterpret_cast<const u32x4*>(k + c) : u32x4{};
+        }
+        float sum = 0.0f;
+        for (int r0 = 0; r0 < wrows; r0 += 32) {
+            const int r = min(r0 + n, wrows - 1);
+            const uint16_t* q = p.q + b * p.qs.b + (int64_t)(r / p.pack) * p.qs.r +
+                                (int64_t)(hb * p.pack + r % p.pack) * p.qs.h;
+            f32x16 s = {};
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                const int c = 16 * t + 8 * h;
+                const u32x4 qf = c < p.D ? *reinterpret_cast<const u32x4*>(q + c) : u32x4{};
+                s = mfma32<BF>(qf, kf[t], s);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int row = r0 + 8 * (i / 4) + 4 * h + i % 4;
+                if (row < wrows) {
+                    const int t = row / p.pack;
+                    const bool sees = j < len.k && (p.tree ? j < len.old || (p.tree[b * (int64_t)p.Sq + t] >> ((j - len.old) & 63) & 1)
+                                                           : j <= len.old + t);
+                    const float x = CAP ? capped(s[i] * yscale, p.cap) : s[i];
+                    const f32x2 ml = *reinterpret_cast<const f32x2*>(row_ml + row * 2);
+                    sum += sees ? __builtin_amdgcn_exp2f(x * f - ml[0]) * ml[1] : 0.0f;
+                }
+            }
+        }
+        sum = half_sum(sum);
+        if (j < len.k && h == 0) weight[(int64_t)bh * p.Sk + j] += sum;
+    }
+}
+
+template <int D, bool BF>
+static hipError_t launch_few(const AttnParams& p, hipStream_t st) {
+    const dim3 g(p.B * p.heads * p.splits), t(256);
+    const bool split = p.splits > 1 || p.row_ml;
+    if (p.cap > 0.0f) {
+        if (split) hipLaunchKernelGGL((attn_few_kernel<D, BF, kCap | kSplit>), g, t, 0, st, p);
+        else hipLaunchKernelGGL((attn_few_kernel<D, BF, kCap>), g, t, 0, st, p);
+    } else {
+        if (split) hipLaunchKernelGGL((attn_few_kernel<D, BF, kSplit>), g, t, 0, st, p);
+        else hipLaunchKernelGGL((attn_few_kernel<D, BF, 0>), g, t, 0, st, p);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_attn_few(AttnParams p, hipStream_t st) {
+    if (p.D > 64) return p.bf16 ? launch_few<128, true>(p, st) : launch_few<128, false>(p, st);
+    return p.bf16 ? launch_few<64, true>(p, st) : launch_few<64, false>(p, st);
+}
+
+hipError_t launch_attn_combine(const AttnParams& p, hipStream_t st) {
+    const dim3 g(p.B * p.heads * p.Sq * p.pack), t(256);
+    if (p.D > 64) {
+        if (p.bf16) hipLaunchKernelGGL((attn_combine_kernel<128, true>), g, t, 0, st, p);
+        else hipLaunchKernelGGL((attn_combine_kernel<128, false>), g, t, 0, st, p);
+    } else {
+        if (p.bf16) hipLaunchKernelGGL((attn_combine_kernel<64, true>), g, t, 0, st, p);
+        else hipLaunchKernelGGL((attn_combine_kernel<64, false>), g, t, 0, st, p);
+    }
+    return hipGetLastError();
+}
+
+template <int D, bool BF>
+static hipError_t launch_weights(const AttnParams& p, float* weight, int wrows, hipStream_t st) {
+    const dim3 g(std::min(64, (p.Sk + 127) / 128), p.B * p.heads), t(256);
+    if (p.cap > 0.0f) hipLaunchKernelGGL((attn_weights_kernel<D, BF, true>), g, t, 0, st, p, weight, wrows);
+    else hipLaunchKernelGGL((attn_weights_kernel<D, BF, false>), g, t, 0, st, p, weight, wrows);
+    return hipGetLastError();
+}
+
+hipError_t launch_attn_weights(const AttnParams& p, float* weight, int rows, hipStream_t st) {
+    const int w = rows * p.pack;
+    if (p.D > 64) return p.bf16 ? launch_weights<128, true>(p, weight, w, st) : launch_weights<128, false>(p, weight, w, st);
+    return p.bf16 ? launch_weights<64, true>(p, weight, w, st) : launch_weights<64, false>(p, weight, w, st);
+}
+
+}  // namespace sltx

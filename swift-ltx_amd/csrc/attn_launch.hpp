@@ -1,0 +1,102 @@
+// attn_launch.hpp -- parameter blocks and host launchers of the attention and
+// key/value cache kernels, shared with their C ABI (attn_capi.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+namespace sltx {
+
+// Strides of a [batch, row, head, head_dim] tensor in elements; head_dim is
+// contiguous.
+struct AttnStrides {
+    int64_t b, r, h;
+};
+
+// One attention over B sequences; see attn_seq.hip and attn_few.hip.  A block's
+// rows are (query row i, head g of `pack`) pairs, i * pack + g: pack is 1, or
+// the query heads that share a key/value head.
+struct AttnParams {
+    const uint16_t *q, *k, *v;
+    uint16_t* out;
+    AttnStrides qs, ks, vs, os;
+    int B, Sq, Sk, Hq, Hk, D;
+    int bf16;
+    float scale, cap;           // cap 0: none
+    const float* bias;          // [Hq or 1][bias_n]: bias[clamp(distance + bias_zero)]
+    int64_t bias_h;             // elements between heads (0: one row for all)
+    int bias_n, bias_zero;
+    int causal;
+    const int32_t* prefix;      // [B] keys that every row sees, or null
+    const int32_t *q_docs, *k_docs;   // [B, Sq], [B, Sk] or null
+    const int32_t *q_lens, *k_lens;   // [B] or null
+    // Over a cache: k_lens are the slots before the new tokens, Sk the capacity,
+    // the keys k_lens[b] + Sq; row i stands at key k_lens[b] + i.
+    int cached;
+    const uint64_t* tree;       // [B, Sq] new tokens that row i sees, or null
+    // filled by the launchers
+    int pack, heads, tiles, splits;
+    float* part_o;              // [B][heads][splits][Sq * pack][DT] sums of a split
+    float* part_ml;             // [B][heads][splits][Sq * pack][2] (f m, l)
+    float* row_ml;              // [B][heads][Sq * pack][2] (f m, 1 / l), or null
+};
+
+// Keys and rows of sequence b.  Lengths come from device memory: out of range
+// ones are cut to what the tensors hold.
+struct SeqLens {
+    int q, k;      // rows, keys
+    int shift;     // row i stands at key i + shift
+    int old;       // cached: keys that every row sees
+};
+__device__ __forceinline__ SeqLens seq_lens(const AttnParams& p, int b) {
+    SeqLens s;
+    s.q = p.q_lens ? min(max(p.q_lens[b], 0), p.Sq) : p.Sq;
+    const int k = p.k_lens ? min(max(p.k_lens[b], 0), p.Sk) : p.Sk;
+    s.old = k;
+    s.k = p.cached ? min(k + s.q, p.Sk) : k;
+    s.shift = p.cached ? k : k - s.q;
+    return s;
+}
+
+constexpr int kSeqTileRows = 128;   // query rows of a block of attn_seq.hip
+constexpr int kTileKeys = 64;       // keys of its tiles
+constexpr int kFewRows = 32;        // most rows of a block of attn_few.hip
+constexpr int kFewKeys = 128;       // keys that its four waves take at a time
+
+hipError_t launch_attn_seq(AttnParams p, hipStream_t st);
+hipError_t launch_attn_few(AttnParams p, hipStream_t st);
+// out = sum of the splits' parts, and row_ml where asked for
+hipError_t launch_attn_combine(const AttnParams& p, hipStream_t st);
+// weight[b, head, key] += the weights of the first `rows` query rows, recomputed
+// from row_ml.
+hipError_t launch_attn_weights(const AttnParams& p, float* weight, int rows, hipStream_t st);
+
+// ---- cache ----
+struct CacheParams {
+    uint16_t *k, *v;            // [layers, B, heads, capacity, D]
+    float* weight;              // [layers, B, heads, capacity] or null
+    int32_t* position;          // the same, or null
+    int32_t *length, *next;     // [B]
+    int layers, B, heads, capacity, D;
+};
+struct AppendParams {
+    CacheParams c;
+    int layer;
+    const uint16_t *q, *k, *v;
+    uint16_t* q_out;            // [B, T, Hq, D]
+    AttnStrides qs, ks, vs;
+    int T, Hq, bf16;
+    const float* inv_freq;      // [pairs]
+    int pairs, interleaved;
+    const int32_t* depth;       // [B, T] or null
+};
+hipError_t launch_kv_append(const AppendParams& p, hipStream_t st);
+hipError_t launch_kv_accept(const CacheParams& c, int drafted, const int32_t* path, int path_len,
+                            const int32_t* count, hipStream_t st);
+size_t kv_evict_workspace_bytes(const CacheParams& c, int budget);
+hipError_t launch_kv_evict(const CacheParams& c, int budget, int sinks, int recent, void* ws,
+                           hipStream_t st);
+
+}  // namespace sltx

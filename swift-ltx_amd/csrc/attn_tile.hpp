@@ -1,0 +1,232 @@
+// attn_tile.hpp -- the pieces that the attention kernels share (attn_seq.hip,
+// attn_few.hip): tiles of keys and values in LDS, their MFMA fragments, and the
+// softmax's running maximum.
+//
+// Orientation.  Both products are formed transposed, S^T = K Q^T and
+// O^T = V^T P^T, on 32x32x16 MFMAs.  In their result layout lane l holds
+// column l & 31 (one query row) and the matrix rows 8*(i/4) + 4*(l/32) + i%4,
+// i = 0..15 (16 of 32 keys, or of 32 output columns): a row's maximum and sum
+// are taken within a lane and with lane l ^ 32, and the statistics are one
+// register each.  The registers that hold P^T after S^T's MFMAs are the second
+// product's B fragments as they stand: a contraction may run over its keys in
+// any order that both operands share, and V^T is read from LDS in the order
+// that P^T has (v_frag).
+#pragma once
+
+#include <type_traits>
+
+#include "attn_launch.hpp"
+#include "q4_common.hpp"
+
+namespace sltx {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) char* lds_char_t;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kInf = __builtin_inff();
+
+// ---- tiles in LDS ----
+// A tile is ROWS rows of D values of 16 bits (D = 64 or 128; a head dim below
+// is padded with zeros).  The 16-byte pieces of a row are permuted by the row
+// so that neither way of reading meets a bank twice in a cycle: K rows are read
+// as pieces by 16 consecutive rows at a time, V rows as 4 rows x 16 columns.
+template <int D>
+__device__ __forceinline__ int k_swizzle(int row) {
+    return D == 128 ? row & 15 : (row >> 1) & 7;
+}
+template <int D>
+__device__ __forceinline__ int v_swizzle(int row) {
+    return D == 128 ? (row & 7) << 1 : ((row >> 1) & 3) << 1;
+}
+
+// The copies of one wave into a tile of which it fills INSTR pieces of 1 KB:
+// byte offsets of each lane's piece from the tile's first row in memory.
+// Pieces past the head dim get an offset that the buffer's bounds check turns
+// into zeros, as it does for the rows past the end (tile_rsrc).
+constexpr int kOutside = 0x7fffff00;
+template <int D, bool V, int INSTR>
+struct TileCopy {
+    int off[INSTR];
+    __device__ __forceinline__ void init(int first, int lane, int stride, int head_bytes) {
+        constexpr int P = D / 8;   // pieces of a row
+#pragma unroll
+        for (int i = 0; i < INSTR; ++i) {
+            const int row = (first + i) * (64 / P) + lane / P, p = lane % P;
+            const int c = p ^ (V ? v_swizzle<D>(row) : k_swizzle<D>(row));
+            off[i] = c * 16 < head_bytes ? row * stride + c * 16 : kOutside;
+        }
+    }
+};
+
+// The buffer that holds `rows` rows (at least 1) from `base` on.
+__device__ __forceinline__ u32x4 tile_rsrc(const uint16_t* base, int rows, int stride, int head_bytes) {
+    const uint64_t a = reinterpret_cast<uint64_t>(base);
+    u32x4 r = {(uint32_t)a, (uint32_t)(a >> 32) & 0xffffu, (uint32_t)((rows - 1) * stride + head_bytes),
+               0x00020000u};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_amdgcn_readfirstlane(r[i]);
+    return r;
+}
+
+// One copy of 1 KB, lane l's 16 bytes to lds + 16 l.  Written as asm so that
+// the compiler's wait counts do not know of it: it cannot tell a copy into one
+// stage from a read of another, and would drain every copy before each read.
+// The kernels wait themselves (copies_wait) before the barrier or the read
+// that hands a stage over.  The instruction has no register output; m0 is a
+// reserved register that nothing else in these kernels uses.
+__device__ __forceinline__ void copy_1k(u32x4 rsrc, int off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                 :: "v"(off), "s"(rsrc), "s"(lds) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+    return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_char_t)(p));
+}
+
+__device__ __forceinline__ u32x4 lds_16(uint32_t a) {
+    return *(__attribute__((address_space(3))) const u32x4*)(uintptr_t)(a);
+}
+__device__ __forceinline__ u32x2 lds_tr8(uint32_t a) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                         (__attribute__((address_space(3))) s16x4*)(uintptr_t)(a)));
+}
+
+// Lane addresses of the fragments within a tile at LDS offset 0.
+// K as A operand: lane l holds key l & 31, columns 16 t + 8 (l >> 5) .. + 7.
+template <int D>
+__device__ __forceinline__ uint32_t k_frag_base(int lane) {
+    const int row = lane & 31;
+    return row * (2 * D) + (((lane >> 5) ^ k_swizzle<D>(row)) << 4);
+}
+template <int D>
+__device__ __forceinline__ u32x4 k_frag(uint32_t tile, uint32_t base, int block, int t) {
+    return lds_16(tile + block * (64 * D) + (base ^ (t << 5)));
+}
+// V^T as A operand of 16 keys: lane l holds column 32 db + (l & 31) and, in the
+// order of P^T's registers, keys 8 (j / 4) + 4 (l >> 5) + j % 4, j = 0..7, of 16:
+// two transposing reads of 4 keys each.
+template <int D>
+__device__ __forceinline__ uint32_t v_frag_base(int lane) {
+    const int row = 4 * (lane >> 5) + ((lane >> 2) & 3);
+    return row * (2 * D) + ((((lane >> 4) & 1) << 5) ^ (v_swizzle<D>(row) << 4)) + (lane & 3) * 8;
+}
+template <int D>
+__device__ __forceinline__ u32x4 v_frag(uint32_t tile, uint32_t base, int ks, int db) {
+    const uint32_t a = tile + ks * (32 * D) + (base ^ (db << 6));
+    const u32x2 x = lds_tr8(a), y = lds_tr8(a + 16 * D);
+    return u32x4{x[0], x[1], y[0], y[1]};
+}
+
+// ---- arithmetic ----
+template <bool BF>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (BF)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                       __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                      __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Two values rounded to nearest even.
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const f32x2 v = {a, b};
+    if constexpr (BF) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
+    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+}
+
+// max / sum with the other half of the wave (lane l ^ 32)
+__device__ __forceinline__ float half_max(float x) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+    const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
+}
+
+// cap * tanh(y).  tanh as (1 - e) / (1 + e) with e = exp(-2 |y|), below 0.25,
+// where 1 - e would cancel, as its series to y^9 (next term under 1e-8 of y):
+// within about 2e-7 of the value, so a score of 12 is off by 2e-6.
+__device__ __forceinline__ float capped(float y, float cap) {
+    const float a = fabsf(y), y2 = y * y;
+    const float e = __builtin_amdgcn_exp2f(-2.0f * kLog2e * a);
+    const float big = (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e);
+    const float small = a + a * y2 * (-1.0f / 3 + y2 * (2.0f / 15 + y2 * (-17.0f / 315 + y2 * (62.0f / 2835))));
+    return cap * copysignf(a < 0.25f ? small : big, y);
+}
+
+// ---- non-finite values in masked places ----
+// A masked key has weight 0, but 0 times an infinity or NaN in its V row would
+// still put NaN into rows that do not see it.  In tiles where some row may not
+// see some key, such values are cleared in LDS before the product (clear_values)
+// and added afterwards to the rows that see their key (add_values): they are
+// what such a row's sum comes to.
+template <bool BF>
+__device__ __forceinline__ bool nonfinite(uint32_t x) {   // of the low 16 bits
+    constexpr uint32_t e = BF ? 0x7f80u : 0x7c00u;
+    return (x & e) == e;
+}
+// Clears the non-finite values of a tile's piece (16 bytes at LDS address a);
+// whether there were any.
+template <bool BF>
+__device__ __forceinline__ bool clear_piece(uint32_t a) {
+    u32x4 v = lds_16(a);
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool lo = nonfinite<BF>(v[i]), hi = nonfinite<BF>(v[i] >> 16);
+        v[i] = (lo ? 0 : v[i] & 0xffffu) | (hi ? 0 : v[i] & 0xffff0000u);
+        bad |= lo | hi;
+    }
+    if (bad) *(__attribute__((address_space(3))) u32x4*)(uintptr_t)(a) = v;
+    return bad;
+}
+// Adds the non-finite values of V row `v` to the lane's sums (for lanes whose
+// row sees it).
+template <int D, bool BF>
+__device__ __forceinline__ void add_values(f32x16 (&o)[D / 32], const uint16_t* v, int head_dim, int h, bool sees) {
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = 32 * db + 8 * i + 4 * h;
+            const u32x2 x = *reinterpret_cast<const u32x2*>(v + min(c, head_dim - 4));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t y = x[e / 2] >> (e % 2 * 16) & 0xffffu;
+                const float z = BF ? bf2f((uint16_t)y) : h2f((uint16_t)y);
+                o[db][4 * i + e] += (sees && nonfinite<BF>(y) && c < head_dim) ? z : 0.0f;
+            }
+            __builtin_amdgcn_sched_barrier(0);   // rare: few registers, not speed
+        }
+}
+
+// o += V^T P^T over the KS * 16 keys of the tile at `tile`.
+template <int D, bool BF, int KS>
+__device__ __forceinline__ void weigh_values(f32x16 (&o)[D / 32], const u32x4 (&pf)[KS], uint32_t tile,
+                                             uint32_t base) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int db = 0; db < D / 32; ++db) o[db] = mfma32<BF>(v_frag<D>(tile, base, ks, db), pf[ks], o[db]);
+}
+
+// ---- running softmax of one lane's column ----
+// Weights are exp2(f x - mf), with x the (capped, biased) score and mf = f m.  m
+// follows the row's maximum only once that has grown by more than 8 in the
+// exponent: until then weights are at most 2^8, which 16 bits hold as exactly
+// as 1, and no sum has to be rescaled.  m = -inf: nothing seen so far.
+struct RowState {
+    float m, mf, l;
+};
+
+}  // namespace sltx

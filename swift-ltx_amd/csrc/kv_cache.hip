@@ -1,0 +1,363 @@
+// kv_cache.hip -- what keeps a key/value cache: appending rotated keys and
+// values, accepting drafted tokens, evicting by accumulated attention weight.
+// All of them move bytes: nothing here does arithmetic that counts.
+#include "attn_launch.hpp"
+#include "q4_common.hpp"
+
+namespace sltx {
+
+// ---- append ----
+// A block takes one token: its angles once (in 64 bits: position times
+// frequency loses whole turns in 32 at far positions), then all its heads' q, k
+// and v, 8 values a thread.  Rotated pairs are (i, i + pairs), or (2i, 2i + 1)
+// interleaved; values past 2 pairs pass through.
+template <bool BF>
+__device__ __forceinline__ float widen(uint32_t x) {
+    return BF ? bf2f((uint16_t)x) : h2f((uint16_t)x);
+}
+template <bool BF>
+__device__ __forceinline__ uint32_t narrow(float x) {
+    return BF ? f2bf(x) : f2h(x);
+}
+
+constexpr int kMaxPairs = 64;
+
+template <bool BF>
+__global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p) {
+    __shared__ float cs[kMaxPairs], sn[kMaxPairs];
+    const int t = blockIdx.x % p.T, b = blockIdx.x / p.T;
+    const CacheParams& c = p.c;
+    const int64_t at = (int64_t)c.next[b] + (p.depth ? p.depth[(int64_t)b * p.T + t] : t);
+    const int64_t slot = (int64_t)c.length[b] + t;
+    if (threadIdx.x < p.pairs) {
+        const double turns = (double)at * (double)p.inv_freq[threadIdx.x] * 0.15915494309189535;
+        const float r = (float)(turns - rint(turns));   // of a turn, -0.5 to 0.5
+        sincospif(2.0f * r, &sn[threadIdx.x], &cs[threadIdx.x]);
+    }
+    __syncthreads();
+    const bool fits = slot >= 0 && slot < c.capacity;   // tokens past the capacity are dropped
+    const int chunks = c.D / 8, qn = p.Hq * chunks, kn = c.heads * chunks;
+    const int64_t lb = (int64_t)p.layer * c.B + b;
+    for (int e = threadIdx.x; e < qn + 2 * kn; e += 256) {
+        const uint16_t* src;
+        uint16_t* dst;
+        int col;
+        bool turn = true;
+        if (e < qn) {
+            const int head = e / chunks;
+            col = e % chunks * 8;
+            src = p.q + b * p.qs.b + t * p.qs.r + head * p.qs.h;
+            dst = p.q_out + (((int64_t)b * p.T + t) * p.Hq + head) * c.D;
+        } else {
+            if (!fits) break;
+            const int i = e - qn, v = i >= kn, head = (v ? i - kn : i) / chunks;
+            col = (v ? i - kn : i) % chunks * 8;
+            src = v ? p.v + b * p.vs.b + t * p.vs.r + head * p.vs.h : p.k + b * p.ks.b + t * p.ks.r + head * p.ks.h;
+            dst = (v ? c.v : c.k) + ((lb * c.heads + head) * c.capacity + slot) * c.D;
+            turn = !v;
+        }
+        u32x4 x = *reinterpret_cast<const u32x4*>(src + col);
+        if (turn && col < 2 * p.pairs) {
+            float y[8], z[8];   // the values and their pairs' others
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = widen<BF>(x[i / 2] >> (i % 2 * 16) & 0xffffu);
+            if (p.interleaved) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) z[i] = y[i ^ 1];
+            } else if (p.pairs % 8 == 0) {
+                const u32x4 o = *reinterpret_cast<const u32x4*>(src + (col < p.pairs ? col + p.pairs : col - p.pairs));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) z[i] = widen<BF>(o[i / 2] >> (i % 2 * 16) & 0xffffu);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int a = col + i;
+                    z[i] = a < 2 * p.pairs ? widen<BF>(src[a < p.pairs ? a + p.pairs : a - p.pairs]) : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int a = col + i;
+                if (a < 2 * p.pairs) {
+                    const int pair = p.interleaved ? a / 2 : a < p.pairs ? a : a - p.pairs;
+                    const bool first = p.interleaved ? a % 2 == 0 : a < p.pairs;
+                    y[i] = y[i] * cs[pair] + (first ? -z[i] : z[i]) * sn[pair];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = narrow<BF>(y[2 * i]) | narrow<BF>(y[2 * i + 1]) << 16;
+        }
+        *reinterpret_cast<u32x4*>(dst + col) = x;
+    }
+    if (c.weight && fits && threadIdx.x < 64)
+        for (int head = threadIdx.x; head < c.heads; head += 64) {
+            const int64_t i = (lb * c.heads + head) * c.capacity + slot;
+            c.weight[i] = 0.0f;
+            c.position[i] = (int32_t)at;
+        }
+}
+
+hipError_t launch_kv_append(const AppendParams& p, hipStream_t st) {
+    const int64_t blocks = (int64_t)p.c.B * p.T;
+    if (blocks == 0) return hipSuccess;
+    if (blocks > 0x7fffff00 / 256) return hipErrorInvalidValue;
+    const dim3 g((unsigned)blocks), t(256);
+    if (p.bf16) hipLaunchKernelGGL(kv_append_kernel<true>, g, t, 0, st, p);
+    else hipLaunchKernelGGL(kv_append_kernel<false>, g, t, 0, st, p);
+    return hipGetLastError();
+}
+
+// ---- accept ----
+constexpr int kMaxPath = 64;
+
+// The tokens of sequence b's path that are accepted: its first count[b], as far
+// as they name drafted tokens that are in the cache.  One wave; all lanes.
+__device__ __forceinline__ int accepted(const CacheParams& c, int b, int drafted, const int32_t* path,
+                                        int path_len, const int32_t* count, int* node) {
+    const int lane = threadIdx.x & 63;
+    const int most = count ? min(max(count[b], 0), path_len) : path_len;
+    const int length = c.length[b];
+    *node = lane < path_len ? path ? path[(int64_t)b * path_len + lane] : lane : -1;
+    const bool good = lane < most && *node >= 0 && *node < drafted && (int64_t)length + *node < c.capacity &&
+                      length >= 0;
+    const uint64_t bad = ~__ballot(good);
+    return bad ? __builtin_ctzll(bad) : 64;
+}
+
+// One block for each layer, sequence and head: the accepted rows are all read
+// before the first is written, so any order of the path is safe.
+__global__ __launch_bounds__(256) void kv_accept_kernel(CacheParams c, int drafted, const int32_t* path,
+                                                        int path_len, const int32_t* count) {
+    __shared__ int nodes[kMaxPath];
+    const int lbh = blockIdx.x, b = lbh / c.heads % c.B;
+    int node;
+    const int n = accepted(c, b, drafted, path, path_len, count, &node);
+    if (threadIdx.x < 64) nodes[threadIdx.x] = node;
+    __syncthreads();
+    const int chunks = c.D / 8;
+    const int64_t row0 = (int64_t)lbh * c.capacity + c.length[b];
+    constexpr int MOST = kMaxPath * 16 / 256;   // 16-byte pieces of a thread, head_dim 128
+    u32x4 kr[MOST], vr[MOST];
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+        const int e = i * 256 + threadIdx.x, r = e / chunks;
+        if (r < n && nodes[r] != r) {
+            const int64_t s = (row0 + nodes[r]) * c.D + e % chunks * 8;
+            kr[i] = *reinterpret_cast<const u32x4*>(c.k + s);
+            vr[i] = *reinterpret_cast<const u32x4*>(c.v + s);
+        }
+    }
+    float w = 0.0f;
+    int32_t at = 0;
+    const int r1 = threadIdx.x;
+    if (c.weight && r1 < n) w = c.weight[row0 + nodes[r1]], at = c.position[row0 + nodes[r1]];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MOST; ++i) {
+        const int e = i * 256 + threadIdx.x, r = e / chunks;
+        if (r < n && nodes[r] != r) {
+            const int64_t d = (row0 + r) * c.D + e % chunks * 8;
+            *reinterpret_cast<u32x4*>(c.k + d) = kr[i];
+            *reinterpret_cast<u32x4*>(c.v + d) = vr[i];
+        }
+    }
+    if (c.weight && r1 < n) c.weight[row0 + r1] = w, c.position[row0 + r1] = at;
+}
+
+// Lengthens the sequences; a launch of its own, after every block has read the
+// old lengths.
+__global__ __launch_bounds__(64) void kv_advance_kernel(CacheParams c, int drafted, const int32_t* path,
+                                                        int path_len, const int32_t* count) {
+    const int b = blockIdx.x;
+    int node;
+    const int n = accepted(c, b, drafted, path, path_len, count, &node);
+    if (threadIdx.x == 0) {
+        c.length[b] += n;
+        c.next[b] += n;
+    }
+}
+__global__ __launch_bounds__(256) void kv_advance_chain_kernel(CacheParams c, int drafted, const int32_t* count) {
+    const int b = blockIdx.x * 256 + threadIdx.x;
+    if (b >= c.B) return;
+    const int length = c.length[b];
+    int n = count ? min(max(count[b], 0), drafted) : drafted;
+    n = max(0, min(n, c.capacity - length));
+    c.length[b] = length + n;
+    c.next[b] += n;
+}
+
+hipError_t launch_kv_accept(const CacheParams& c, int drafted, const int32_t* path, int path_len,
+                            const int32_t* count, hipStream_t st) {
+    if (c.B == 0) return hipSuccess;
+    if (!path) {
+        hipLaunchKernelGGL(kv_advance_chain_kernel, dim3((c.B + 255) / 256), dim3(256), 0, st, c, drafted, count);
+        return hipGetLastError();
+    }
+    const int64_t blocks = (int64_t)c.layers * c.B * c.heads;
+    if (blocks > 0x7fffff00 / 256) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(kv_accept_kernel, dim3((unsigned)blocks), dim3(256), 0, st, c, drafted, path, path_len, count);
+    hipLaunchKernelGGL(kv_advance_kernel, dim3(c.B), dim3(64), 0, st, c, drafted, path, path_len, count);
+    return hipGetLastError();
+}
+
+// ---- evict ----
+// Which entries stay is a selection of the `budget` largest keys: the weight as
+// an unsigned number of the same order (NaN lowest, -0 as 0), the largest of all
+// for protected positions; of equal keys the lowest slots.  A radix select over
+// four digits of 8 bits, then one pass in slot order for the holes (slots below
+// the budget whose entry goes) and the comers (entries from slots above it that
+// stay), which a second launch moves into them.
+constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
+
+struct EvictParams {
+    CacheParams c;
+    int budget, sinks, recent;
+    int32_t *moves, *holes, *comers;   // [layers * B * heads], [...][most] twice
+    int most;
+};
+
+__device__ __forceinline__ uint32_t evict_key(const EvictParams& p, int64_t i, int64_t after) {
+    const int32_t at = p.c.position[i];
+    if (at < p.sinks || (int64_t)at >= after - p.recent) return 0xffffffffu;
+    const float w = p.c.weight[i];
+    if (w != w) return 0;
+    const uint32_t u = __float_as_uint(w + 0.0f);
+    return u >> 31 ? ~u : u | 0x80000000u;
+}
+
+__global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictParams p) {
+    __shared__ int hist[256];
+    __shared__ int sums[kEvictWaves][2];
+    __shared__ int found[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int lbh = blockIdx.x, b = lbh / p.c.heads % p.c.B;
+    const int n = min(p.c.length[b], p.c.capacity);
+    if (n <= p.budget) {
+        if (tid == 0) p.moves[lbh] = 0;
+        return;
+    }
+    const int64_t after = p.c.next[b], base = (int64_t)lbh * p.c.capacity;
+    uint32_t prefix = 0;
+    int want = p.budget;   // of the keys that start with the prefix
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        if (tid < 256) hist[tid] = 0;
+        __syncthreads();
+        for (int s = tid; s < n; s += kEvictThreads) {
+            const uint32_t k = evict_key(p, base + s, after);
+            if (shift == 24 || k >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&hist[k >> shift & 255], 1);
+        }
+        __syncthreads();
+        if (wave == 0) {   // the digit in which the count from the top reaches `want`
+            int c[4], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum += c[i] = hist[255 - (lane * 4 + i)];
+            int before = sum;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int x = __shfl_up(before, o, 64);
+                if (lane >= o) before += x;
+            }
+            before -= sum;
+            if (before < want && before + sum >= want) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (before < want && before + c[i] >= want) {
+                        found[0] = 255 - (lane * 4 + i);
+                        found[1] = want - before;
+                        break;
+                    }
+                    before += c[i];
+                }
+            }
+        }
+        __syncthreads();
+        prefix |= (uint32_t)found[0] << shift;
+        want = found[1];
+        __syncthreads();
+    }
+    // `prefix` is the smallest key that stays; `want` of the entries with it do.
+    // Each wave takes a run of slots, a multiple of 64.
+    const int run = (n + kEvictThreads - 1) / kEvictThreads * 64;
+    const int s0 = wave * run, s1 = min(n, s0 + run);
+    const uint64_t below = (1ull << lane) - 1;
+    int ties = 0;
+    for (int s = s0; s < s1; s += 64)
+        ties += __popcll(__ballot(s + lane < s1 && evict_key(p, base + s + lane, after) == prefix));
+    if (lane == 0) sums[wave][0] = ties;
+    __syncthreads();
+    int tie0 = 0;
+    for (int w = 0; w < wave; ++w) tie0 += sums[w][0];
+    __syncthreads();
+    for (int pass = 0; pass < 2; ++pass) {   // count, then write
+        int tie = tie0, hole = 0, comer = 0;
+        if (pass == 1)
+            for (int w = 0; w < wave; ++w) hole += sums[w][0], comer += sums[w][1];
+        for (int s = s0; s < s1; s += 64) {
+            const int slot = s + lane;
+            const uint32_t k = slot < s1 ? evict_key(p, base + slot, after) : 0;
+            const uint64_t t = __ballot(slot < s1 && k == prefix);
+            const bool keep = slot < s1 && (k > prefix || (k == prefix && tie + __popcll(t & below) < want));
+            tie += __popcll(t);
+            const bool is_hole = slot < s1 && slot < p.budget && !keep, is_comer = keep && slot >= p.budget;
+            const uint64_t hm = __ballot(is_hole), cm = __ballot(is_comer);
+            if (pass == 1) {
+                if (is_hole) p.holes[(int64_t)lbh * p.most + hole + __popcll(hm & below)] = slot;
+                if (is_comer) p.comers[(int64_t)lbh * p.most + comer + __popcll(cm & below)] = slot;
+            }
+            hole += __popcll(hm);
+            comer += __popcll(cm);
+        }
+        if (pass == 0) {
+            if (lane == 0) sums[wave][0] = hole, sums[wave][1] = comer;
+            __syncthreads();
+        } else if (wave == kEvictWaves - 1 && lane == 0) {
+            p.moves[lbh] = hole;
+        }
+    }
+}
+
+// Moves the comers into the holes: disjoint slots, in any order.  A row's pieces
+// go to neighbouring lanes.
+__global__ __launch_bounds__(256) void kv_evict_move_kernel(EvictParams p) {
+    const int lbh = blockIdx.y, b = lbh / p.c.heads % p.c.B;
+    const int chunks = p.c.D / 8, moves = p.moves[lbh];
+    const int32_t *holes = p.holes + (int64_t)lbh * p.most, *comers = p.comers + (int64_t)lbh * p.most;
+    const int64_t base = (int64_t)lbh * p.c.capacity;
+    for (int e = blockIdx.x * 256 + threadIdx.x; e < moves * chunks; e += gridDim.x * 256) {
+        const int m = e / chunks, piece = e % chunks;
+        const int64_t d = base + holes[m], s = base + comers[m];
+        const u32x4 k = *reinterpret_cast<const u32x4*>(p.c.k + s * p.c.D + piece * 8);
+        const u32x4 v = *reinterpret_cast<const u32x4*>(p.c.v + s * p.c.D + piece * 8);
+        *reinterpret_cast<u32x4*>(p.c.k + d * p.c.D + piece * 8) = k;
+        *reinterpret_cast<u32x4*>(p.c.v + d * p.c.D + piece * 8) = v;
+        if (piece == 0) {
+            p.c.weight[d] = p.c.weight[s];
+            p.c.position[d] = p.c.position[s];
+        }
+    }
+    // no block of this launch reads the lengths
+    if (blockIdx.x == 0 && threadIdx.x == 0 && lbh / p.c.heads / p.c.B == 0 && lbh % p.c.heads == 0)
+        p.c.length[b] = min(p.c.length[b], p.budget);
+}
+
+size_t kv_evict_workspace_bytes(const CacheParams& c, int budget) {
+    const size_t lbh = (size_t)c.layers * c.B * c.heads;
+    return lbh * (1 + 2 * (size_t)std::min(budget, c.capacity - budget)) * sizeof(int32_t);
+}
+
+hipError_t launch_kv_evict(const CacheParams& c, int budget, int sinks, int recent, void* ws, hipStream_t st) {
+    const int64_t lbh = (int64_t)c.layers * c.B * c.heads;
+    if (lbh == 0 || budget == c.capacity) return hipSuccess;
+    if (lbh > 65535) return hipErrorInvalidValue;
+    EvictParams p = {c, budget, sinks, recent, nullptr, nullptr, nullptr, std::min(budget, c.capacity - budget)};
+    p.moves = static_cast<int32_t*>(ws);
+    p.holes = p.moves + lbh;
+    p.comers = p.holes + lbh * p.most;
+    hipLaunchKernelGGL(kv_evict_select_kernel, dim3((unsigned)lbh), dim3(kEvictThreads), 0, st, p);
+    const int64_t pieces = (int64_t)p.most * (c.D / 8);
+    const unsigned x = (unsigned)std::max<int64_t>(1, std::min<int64_t>((pieces + 255) / 256, (2048 + lbh - 1) / lbh));
+    hipLaunchKernelGGL(kv_evict_move_kernel, dim3(x, (unsigned)lbh), dim3(256), 0, st, p);
+    return hipGetLastError();
+}
+
+}  // namespace sltx

@@ -437,6 +437,9 @@ SampleParams sample_params(const void* logits, int dtype, int n, float temperatu
 }
 
 }  // namespace
+
+int require_device() { return ensure_device(); }
+
 }  // namespace sltx
 
 using namespace sltx;
