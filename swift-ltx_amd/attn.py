@@ -21,11 +21,16 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
+import sys
+
+_P = sys.modules[__package__]
 
 
-def _pkg():
-    import swiftltx_amd
-    return swiftltx_amd
+def _native():
+    """The native binding of the plain calls (csrc/py/q4_binding.cpp), or None."""
+    if not _P._native_tried:
+        _P._load_binding()
+    return _P._native
 
 
 @contextlib.contextmanager
@@ -102,8 +107,13 @@ def attention(q, k, v, scale, *, softcap=0.0, bias=None, bias_zero=0, causal=Fal
     causal or j <= pos or j < prefix, and both are of one document (negative ids:
     of none).  A row that sees nothing gives zeros; rows from q_len on are left as
     they are in `out` (default: a new tensor; with q_lens its last rows are zeros)."""
+    native = _native()
+    if native is not None:
+        r = native.attention(q, k, v, scale, softcap, bias, bias_zero, causal, prefix, q_docs, k_docs, q_lens, k_lens,
+                             out, stream)
+        if r is not None:
+            return r
     import torch
-    P = _pkg()
     if q is None or q.dim() != 4 or k is None or k.dim() != 4:
         raise ValueError("q and k are [batch, rows, heads, head_dim] tensors")
     if q.dtype not in _halves():
@@ -114,8 +124,8 @@ def attention(q, k, v, scale, *, softcap=0.0, bias=None, bias_zero=0, causal=Fal
     _rows(q, "q", (B, Sq, Hq, D), q.dtype, None)
     _rows(k, "k", (B, Sk, Hk, D), q.dtype, dev)
     _rows(v, "v", (B, Sk, Hk, D), q.dtype, dev)
-    a = P.CAttentionArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_stride=_strides(q), k_stride=_strides(k),
-                         v_stride=_strides(v), dtype=P._dtype_code(q.dtype), batch=B, q_rows=Sq, k_rows=Sk,
+    a = _P.CAttentionArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_stride=_strides(q), k_stride=_strides(k),
+                         v_stride=_strides(v), dtype=_P._dtype_code(q.dtype), batch=B, q_rows=Sq, k_rows=Sk,
                          q_heads=Hq, kv_heads=Hk, head_dim=D, causal=1 if causal else 0, scale=scale,
                          softcap=softcap)
     if bias is not None:
@@ -136,7 +146,7 @@ def attention(q, k, v, scale, *, softcap=0.0, bias=None, bias_zero=0, causal=Fal
             out = new(B, Sq, Hq, D, dtype=q.dtype, device=dev)
         _rows(out, "out", (B, Sq, Hq, D), q.dtype, dev)
         a.out, a.out_stride = out.data_ptr(), _strides(out)
-        P.check(P.lib().sltx_attention(ctypes.byref(a), handle))
+        _P.check(_P.lib().sltx_attention(ctypes.byref(a), handle))
     return out
 
 
@@ -177,7 +187,6 @@ class KVCache:
 
     def _set(self, k, v, counts, weight, position):
         import torch
-        P = _pkg()
         if k.dim() != 5:
             raise ValueError("k is [layers, batch, kv_heads, capacity, head_dim]")
         _need(k, "k", k.shape, _halves())
@@ -194,19 +203,19 @@ class KVCache:
         self.dtype, self.device = k.dtype, k.device
         self._scratch = []        # the last one is in use; earlier ones a captured graph may name
         self._needs = {}          # bytes of scratch by call
-        self.c = P.CKVCache(k.data_ptr(), v.data_ptr(), P._ptr(weight), P._ptr(position), self.length.data_ptr(),
-                            self.next_position.data_ptr(), *k.shape, P._dtype_code(k.dtype), None, 0)
+        self.c = _P.CKVCache(k.data_ptr(), v.data_ptr(), _P._ptr(weight), _P._ptr(position), self.length.data_ptr(),
+                            self.next_position.data_ptr(), *k.shape, _P._dtype_code(k.dtype), None, 0)
         self._ref = ctypes.byref(self.c)
+        self._handle = (ctypes.addressof(self.c), self.device.index)
 
     def _workspace(self, name, *args):
         """Scratch for the call, of the size its query names (on the current stream)."""
-        P = _pkg()
         key = (name, *args)
         need = self._needs.get(key)
         if need is None:
-            need = int(getattr(P.lib(), name)(self._ref, *args))
+            need = int(getattr(_P.lib(), name)(self._ref, *args))
             if need < 0:
-                P.check(need)
+                _P.check(need)
             self._needs[key] = need
         if need > self.c.workspace_bytes:
             import torch
@@ -225,8 +234,12 @@ def attention_cached(q, cache, layer, scale, *, softcap=0.0, tree=None, weight_r
     entries and the new tokens up to itself, or with `tree` (int64 [batch, T], T <=
     64) those whose bit is set in tree[b, t] (tree_masks).  weight_rows: adds the
     attention weights of the first so many tokens to cache.weight (T <= 64)."""
+    native = _native()
+    if native is not None:
+        r = native.attention_cached(q, *cache._handle, layer, scale, softcap, tree, weight_rows, out, stream)
+        if r is not None:
+            return r
     import torch
-    P = _pkg()
     if q is None or q.dim() != 4:
         raise ValueError("q is a [batch, tokens, q_heads, head_dim] tensor")
     B, T, Hq, D = q.shape
@@ -237,7 +250,7 @@ def attention_cached(q, cache, layer, scale, *, softcap=0.0, tree=None, weight_r
             out = torch.empty(B, T, Hq, D, dtype=q.dtype, device=q.device)
         _need(out, "out", q.shape, (q.dtype,), q.device)
         cache._workspace("sltx_attention_cached_workspace", T, Hq, weight_rows)
-        P.check(P.lib().sltx_attention_cached(q.data_ptr(), _strides(q), cache._ref, layer, T, Hq, scale, softcap,
+        _P.check(_P.lib().sltx_attention_cached(q.data_ptr(), _strides(q), cache._ref, layer, T, Hq, scale, softcap,
                                               tree, weight_rows, out.data_ptr(), handle))
     return out
 
@@ -249,8 +262,12 @@ def kv_append(q, k, v, cache, layer, inv_freq=None, *, depth=None, interleaved=F
     1, ...: a chain).  Returns the rotated q (contiguous).  Pairs of values are (i,
     i + pairs), or (2i, 2i + 1) if interleaved.  The tokens count once they are
     accepted (kv_accept), after every layer has them."""
+    native = _native()
+    if native is not None:
+        r = native.kv_append(q, k, v, *cache._handle, layer, inv_freq, depth, interleaved, q_out, stream)
+        if r is not None:
+            return r
     import torch
-    P = _pkg()
     if q is None or q.dim() != 4:
         raise ValueError("q is a [batch, tokens, q_heads, head_dim] tensor")
     B, T, Hq, D = q.shape
@@ -266,7 +283,7 @@ def kv_append(q, k, v, cache, layer, inv_freq=None, *, depth=None, interleaved=F
         if q_out is None:
             q_out = torch.empty(B, T, Hq, D, dtype=q.dtype, device=q.device)
         _need(q_out, "q_out", q.shape, (q.dtype,), q.device)
-        P.check(P.lib().sltx_kv_append(q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(),
+        _P.check(_P.lib().sltx_kv_append(q.data_ptr(), _strides(q), k.data_ptr(), _strides(k), v.data_ptr(),
                                        _strides(v), cache._ref, layer, T, Hq, inv_freq, pairs,
                                        1 if interleaved else 0, depth, q_out.data_ptr(), handle))
     return q_out
@@ -277,8 +294,10 @@ def kv_accept(cache, drafted, path=None, count=None, stream=None):
     n <= 64: indices among the drafted, root first), the first count[b] of them
     (int32 [batch]; None: all), become the sequences' next entries; without a path
     the first count[b] (None: all) drafted tokens."""
+    native = _native()
+    if native is not None and native.kv_accept(*cache._handle, drafted, path, count, stream):
+        return
     import torch
-    P = _pkg()
     n = 0
     if path is not None:
         if path.dim() != 2:
@@ -287,7 +306,7 @@ def kv_accept(cache, drafted, path=None, count=None, stream=None):
         path = _need(path, "path", (cache.batch, n), (torch.int32,), cache.device).data_ptr()
     count = _opt(count, "count", (cache.batch,), torch.int32, cache.device)
     with _launch(cache.k, stream) as handle:
-        P.check(P.lib().sltx_kv_accept(cache._ref, drafted, path, n, count, handle))
+        _P.check(_P.lib().sltx_kv_accept(cache._ref, drafted, path, n, count, handle))
 
 
 def kv_evict(cache, budget, *, sinks=4, recent=32, stream=None):
@@ -295,10 +314,12 @@ def kv_evict(cache, budget, *, sinks=4, recent=32, stream=None):
     the first `sinks` and the last `recent` positions stay, and of the rest those
     with the highest accumulated attention weight (ties: the lower slots).  Entries
     that stay move only into slots that became free."""
-    P = _pkg()
+    native = _native()
+    if native is not None and native.kv_evict(*cache._handle, budget, sinks, recent, stream):
+        return
     with _launch(cache.k, stream) as handle:
         cache._workspace("sltx_kv_evict_workspace", budget)
-        P.check(P.lib().sltx_kv_evict(cache._ref, budget, sinks, recent, handle))
+        _P.check(_P.lib().sltx_kv_evict(cache._ref, budget, sinks, recent, handle))
 
 
 # ---- what a program prepares once ----

@@ -377,10 +377,10 @@ int sltx_kv_evict(const sltx_kv_cache* cache, int32_t budget, int32_t sinks, int
     const char* fn = "sltx_kv_evict";
     int rc = check_cache(fn, cache);
     if (rc != kOk || (rc = check_evict(fn, cache, budget)) != kOk) return rc;
+    if (cache->batch > 0 && !cache->weight) return set_error(kErrInvalid, "%s: the cache has no weight", fn);
     if (sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)
         return set_error(kErrInvalid, "%s: %d first and %d recent positions in a budget of %d", fn, sinks, recent, budget);
     if (cache->batch == 0) return kOk;
-    if (!cache->weight) return set_error(kErrInvalid, "%s: the cache has no weight", fn);
     const CacheParams c = cache_params(cache);
     if ((rc = need_workspace(fn, cache, kv_evict_workspace_bytes(c, budget))) != kOk) return rc;
     if ((rc = require_device()) != kOk) return rc;

@@ -13,6 +13,8 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <algorithm>
+
 #include <ATen/ATen.h>
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
@@ -20,6 +22,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include "swiftltx_attention.h"
 #include "swiftltx_q4.h"
 
 namespace {
@@ -30,7 +33,9 @@ namespace {
     X(sltx_linear) X(sltx_matmul_q4_silu_mul) X(sltx_matmul_q4_ex) X(sltx_matmul_q4_geglu)        \
     X(sltx_embedding_q4) X(sltx_rms_norm) X(sltx_residual_rms_norm) X(sltx_rmsnorm_matmul_q4)     \
     X(sltx_residual_rmsnorm_matmul_q4_silu_mul) X(sltx_matmul_q4_residual)                        \
-    X(sltx_matmul_q4_residual_rms_norm) X(sltx_argmax) X(sltx_sample_top_p)
+    X(sltx_matmul_q4_residual_rms_norm) X(sltx_argmax) X(sltx_sample_top_p)                       \
+    X(sltx_attention) X(sltx_attention_cached) X(sltx_attention_cached_workspace)                 \
+    X(sltx_kv_append) X(sltx_kv_accept) X(sltx_kv_evict) X(sltx_kv_evict_workspace)
 #define X(name) decltype(&name) f_##name = nullptr;
 SLTX_ENTRIES(X)
 #undef X
@@ -474,6 +479,206 @@ ENTRY(py_sample) {
     });
 }
 
+// ---- attention and the key/value cache ----
+// These allocate only on the current stream of the tensors' device: a call on
+// another stream is made here where its output is given, else declined.
+
+// A [batch, rows, heads, head_dim] tensor with contiguous rows of head_dim, its
+// strides (0 for dimensions that are never stepped over).
+struct Rows {
+    void* p;
+    int64_t size[4], stride[3];
+    at::ScalarType type;
+    int device;
+};
+Rows rows_of(PyObject* o) {
+    const at::Tensor& t = tensor(o);
+    need(t.is_cuda() && t.dim() == 4 && t.numel() > 0 && (t.size(3) == 1 || t.stride(3) == 1));
+    Rows r;
+    for (int i = 0; i < 4; ++i) {
+        r.size[i] = t.size(i);
+        need(r.size[i] <= INT32_MAX);
+        if (i < 3) r.stride[i] = r.size[i] == 1 ? 0 : t.stride(i);
+    }
+    r.type = t.scalar_type();
+    need(r.type == at::kHalf || r.type == at::kBFloat16);
+    r.device = t.get_device();
+    r.p = t.data_ptr();
+    return r;
+}
+void need_like(const Rows& r, int64_t batch, int64_t rows, int64_t heads, int64_t dim, at::ScalarType type, int device) {
+    need(r.size[0] == batch && r.size[1] == rows && r.size[2] == heads && r.size[3] == dim && r.type == type &&
+         r.device == device);
+}
+// None, or a contiguous device tensor of these sizes.
+const void* optional(PyObject* o, at::ScalarType d, int device, int64_t n0, int64_t n1 = -1) {
+    if (o == Py_None) return nullptr;
+    const at::Tensor& t = tensor(o);
+    need(t.dim() == (n1 < 0 ? 1 : 2) && t.size(0) == n0 && (n1 < 0 || t.size(1) == n1) && t.is_cuda() &&
+         t.get_device() == device);
+    return data(t, d, t.numel());
+}
+// The stream of a call on tensors of `device`, which has to be the current one;
+// what the call allocates has to come from that stream.
+void* stream_on(PyObject* o, int device, bool allocates) {
+    const c10::hip::HIPStream cur = c10::hip::getCurrentHIPStream();
+    need(cur.device_index() == device);
+    if (o == Py_None) return cur.stream();
+    void* st = stream(o);
+    need(!allocates || st == cur.stream());
+    return st;
+}
+// The structure that a KVCache keeps, by its address and its tensors' device.
+const sltx_kv_cache* cache_of(PyObject* addr, PyObject* dev, int* device) {
+    need(PyLong_CheckExact(addr));
+    const auto* c = static_cast<const sltx_kv_cache*>(PyLong_AsVoidPtr(addr));
+    need(c && !PyErr_Occurred());
+    *device = i32(dev);
+    return c;
+}
+at::ScalarType cache_type(const sltx_kv_cache* c) { return c->dtype == SLTX_BF16 ? at::kBFloat16 : at::kHalf; }
+
+// q, k, v, scale, softcap, bias, bias_zero, causal, prefix, q_docs, k_docs, q_lens, k_lens, out, stream
+ENTRY(py_attention) {
+    return guarded(n, 15, [&]() -> PyObject* {
+        const Rows q = rows_of(a[0]), k = rows_of(a[1]), v = rows_of(a[2]);
+        need_like(k, q.size[0], k.size[1], k.size[2], q.size[3], q.type, q.device);
+        need_like(v, q.size[0], k.size[1], k.size[2], q.size[3], q.type, q.device);
+        need(a[7] == Py_True || a[7] == Py_False);
+        need(a[13] != Py_None || a[11] == Py_None);   // rows past q_lens of a new output are zeroed first
+        sltx_attention_args g{};
+        g.q = q.p, g.k = k.p, g.v = v.p;
+        g.dtype = dtype_code(q.type);
+        g.batch = (int32_t)q.size[0], g.q_rows = (int32_t)q.size[1], g.k_rows = (int32_t)k.size[1];
+        g.q_heads = (int32_t)q.size[2], g.kv_heads = (int32_t)k.size[2], g.head_dim = (int32_t)q.size[3];
+        g.scale = f32(a[3]), g.softcap = f32(a[4]);
+        g.causal = a[7] == Py_True;
+        if (a[5] != Py_None) {
+            const at::Tensor& b = tensor(a[5]);
+            need(b.dim() == 2 && (b.size(0) == 1 || b.size(0) == q.size[2]) && b.size(1) > 0 && b.size(1) <= INT32_MAX &&
+                 b.get_device() == q.device);
+            g.bias = static_cast<const float*>(data(b, at::kFloat, b.numel()));
+            g.bias_len = (int32_t)b.size(1), g.bias_zero = i32(a[6]);
+            g.bias_head_stride = b.size(0) == 1 ? 0 : b.size(1);
+        }
+        const int64_t B = q.size[0];
+        g.prefix = static_cast<const int32_t*>(optional(a[8], at::kInt, q.device, B));
+        g.q_docs = static_cast<const int32_t*>(optional(a[9], at::kInt, q.device, B, q.size[1]));
+        g.k_docs = static_cast<const int32_t*>(optional(a[10], at::kInt, q.device, B, k.size[1]));
+        g.q_lens = static_cast<const int32_t*>(optional(a[11], at::kInt, q.device, B));
+        g.k_lens = static_cast<const int32_t*>(optional(a[12], at::kInt, q.device, B));
+        void* st = stream_on(a[14], q.device, a[13] == Py_None);
+        Out out;
+        if (a[13] == Py_None) {
+            out.set(a[13], q.size, q.type, tensor(a[0]));
+            g.out_stride[2] = q.size[3];
+            g.out_stride[1] = q.size[2] * q.size[3];
+            g.out_stride[0] = q.size[1] * g.out_stride[1];
+        } else {
+            const Rows o = rows_of(a[13]);
+            need_like(o, B, q.size[1], q.size[2], q.size[3], q.type, q.device);
+            out.ptr = o.p;
+            Py_INCREF(out.obj = a[13]);
+            std::copy(o.stride, o.stride + 3, g.out_stride);
+        }
+        g.out = out.ptr;
+        std::copy(q.stride, q.stride + 3, g.q_stride);
+        std::copy(k.stride, k.stride + 3, g.k_stride);
+        std::copy(v.stride, v.stride + 3, g.v_stride);
+        return call([&] { return f_sltx_attention(&g, st); }) ? out.give() : nullptr;
+    });
+}
+
+// q, cache, device, layer, scale, softcap, tree, weight_rows, out, stream
+ENTRY(py_attention_cached) {
+    return guarded(n, 10, [&]() -> PyObject* {
+        int device;
+        const sltx_kv_cache* c = cache_of(a[1], a[2], &device);
+        const Rows q = rows_of(a[0]);
+        need_like(q, c->batch, q.size[1], q.size[2], c->head_dim, cache_type(c), device);
+        const int32_t layer = i32(a[3]), rows = i32(a[7]), T = (int32_t)q.size[1], heads = (int32_t)q.size[2];
+        const float scale = f32(a[4]), cap = f32(a[5]);
+        const auto* tree = static_cast<const uint64_t*>(optional(a[6], at::kLong, device, c->batch, T));
+        const int64_t bytes = f_sltx_attention_cached_workspace(c, T, heads, rows);
+        need(bytes >= 0 && (uint64_t)bytes <= c->workspace_bytes);   // else Python grows it
+        void* st = stream_on(a[9], device, a[8] == Py_None);
+        Out out;
+        out.set(a[8], q.size, q.type, tensor(a[0]));
+        if (a[8] != Py_None) need(tensor(a[8]).sizes() == at::IntArrayRef(q.size, 4) && tensor(a[8]).get_device() == device);
+        return call([&] {
+                   return f_sltx_attention_cached(q.p, q.stride, c, layer, T, heads, scale, cap, tree, rows, out.ptr, st);
+               }) ? out.give() : nullptr;
+    });
+}
+
+// q, k, v, cache, device, layer, inv_freq, depth, interleaved, q_out, stream
+ENTRY(py_kv_append) {
+    return guarded(n, 11, [&]() -> PyObject* {
+        int device;
+        const sltx_kv_cache* c = cache_of(a[3], a[4], &device);
+        const Rows q = rows_of(a[0]), k = rows_of(a[1]), v = rows_of(a[2]);
+        const int64_t T = q.size[1];
+        need_like(q, c->batch, T, q.size[2], c->head_dim, cache_type(c), device);
+        need_like(k, c->batch, T, c->kv_heads, c->head_dim, q.type, device);
+        need_like(v, c->batch, T, c->kv_heads, c->head_dim, q.type, device);
+        need(a[8] == Py_True || a[8] == Py_False);
+        const int32_t layer = i32(a[5]);
+        const float* freq = nullptr;
+        int32_t pairs = 0;
+        if (a[6] != Py_None) {
+            const at::Tensor& f = tensor(a[6]);
+            need(f.dim() == 1 && f.numel() <= INT32_MAX && f.get_device() == device);
+            pairs = (int32_t)f.numel();
+            freq = static_cast<const float*>(data(f, at::kFloat, pairs));
+        }
+        const auto* depth = static_cast<const int32_t*>(optional(a[7], at::kInt, device, c->batch, T));
+        void* st = stream_on(a[10], device, a[9] == Py_None);
+        Out out;
+        out.set(a[9], q.size, q.type, tensor(a[0]));
+        if (a[9] != Py_None) need(tensor(a[9]).sizes() == at::IntArrayRef(q.size, 4) && tensor(a[9]).get_device() == device);
+        const int inter = a[8] == Py_True;
+        return call([&] {
+                   return f_sltx_kv_append(q.p, q.stride, k.p, k.stride, v.p, v.stride, c, layer, (int32_t)T,
+                                           (int32_t)q.size[2], freq, pairs, inter, depth, out.ptr, st);
+               }) ? out.give() : nullptr;
+    });
+}
+
+// cache, device, drafted, path, count, stream -> True
+ENTRY(py_kv_accept) {
+    return guarded(n, 6, [&]() -> PyObject* {
+        int device;
+        const sltx_kv_cache* c = cache_of(a[0], a[1], &device);
+        const int32_t drafted = i32(a[2]);
+        int32_t len = 0;
+        const int32_t* path = nullptr;
+        if (a[3] != Py_None) {
+            const at::Tensor& t = tensor(a[3]);
+            need(t.dim() == 2 && t.numel() > 0 && t.size(1) <= INT32_MAX);
+            len = (int32_t)t.size(1);
+            path = static_cast<const int32_t*>(optional(a[3], at::kInt, device, c->batch, len));
+        }
+        const auto* count = static_cast<const int32_t*>(optional(a[4], at::kInt, device, c->batch));
+        void* st = stream_on(a[5], device, false);
+        if (!call([&] { return f_sltx_kv_accept(c, drafted, path, len, count, st); })) return nullptr;
+        Py_RETURN_TRUE;
+    });
+}
+
+// cache, device, budget, sinks, recent, stream -> True
+ENTRY(py_kv_evict) {
+    return guarded(n, 6, [&]() -> PyObject* {
+        int device;
+        const sltx_kv_cache* c = cache_of(a[0], a[1], &device);
+        const int32_t budget = i32(a[2]), sinks = i32(a[3]), recent = i32(a[4]);
+        const int64_t bytes = f_sltx_kv_evict_workspace(c, budget);
+        need(bytes >= 0 && (uint64_t)bytes <= c->workspace_bytes);
+        void* st = stream_on(a[5], device, false);
+        if (!call([&] { return f_sltx_kv_evict(c, budget, sinks, recent, st); })) return nullptr;
+        Py_RETURN_TRUE;
+    });
+}
+
 // init(addresses by name, check, Q4Weight)
 PyObject* py_init(PyObject*, PyObject* args) {
     PyObject *addr, *check, *type;
@@ -504,6 +709,7 @@ PyMethodDef methods[] = {
     METHOD(rms_norm), METHOD(residual_rms_norm), METHOD(rmsnorm_matmul_q4),
     METHOD(residual_rmsnorm_matmul_q4_silu_mul), METHOD(matmul_q4_residual),
     METHOD(matmul_q4_residual_rms_norm), METHOD(embedding_q4), METHOD(argmax), METHOD(sample),
+    METHOD(attention), METHOD(attention_cached), METHOD(kv_append), METHOD(kv_accept), METHOD(kv_evict),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_q4_binding", nullptr, -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
