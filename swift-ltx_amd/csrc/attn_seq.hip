@@ -20,13 +20,14 @@ struct DocTiles {
 };
 
 template <int D, bool BF, int MODE>
-__global__ __launch_bounds__(256, 2) void attn_seq_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnParams p) {
     constexpr bool CAP = MODE & kCap, BIAS = MODE & kBias, SPLIT = MODE & kSplit;
     constexpr int TILE = kTileKeys * D;          // values of a tile
     constexpr int QT = D / 16, DB = D / 32;
     constexpr int INSTR = TILE * 2 / 1024 / 4;   // copies of a wave into a tile
     __shared__ __attribute__((aligned(1024))) uint16_t ks[2][TILE], vs[2][TILE];
     __shared__ DocTiles docs;
+    __shared__ __attribute__((aligned(16))) int tile_docs[2][kTileKeys];   // [stage]: documents of the keys
     __shared__ uint32_t bad_keys[2][2];   // [stage]: keys whose V rows are not finite
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -82,8 +83,10 @@ __global__ __launch_bounds__(256, 2) void attn_seq_kernel(AttnParams p) {
         last = min(last, first + each);
     }
 
-    // documents of the rows
-    int qdoc = -1, wdoc0 = 0x7fffffff, wdoc1 = -1, bdoc0 = 0, bdoc1 = 0;
+    // documents of the rows: the smallest and largest of a wave's and of the
+    // block's, and the one that all of them are of (-2: none, as where a row is of
+    // no document)
+    int qdoc = -1, wdoc0 = 0x7fffffff, wdoc1 = -1, wdoc = -2, bdoc0 = 0, bdoc1 = 0, bdoc = -2;
     const int32_t* kdocs = nullptr;
     if (p.q_docs) {
         kdocs = p.k_docs + b * (int64_t)p.Sk;
@@ -97,10 +100,15 @@ __global__ __launch_bounds__(256, 2) void attn_seq_kernel(AttnParams p) {
         }
         wdoc0 = __builtin_amdgcn_readfirstlane(wdoc0);
         wdoc1 = __builtin_amdgcn_readfirstlane(wdoc1);
-        if (lane == 0) docs.lo[wave] = wdoc0, docs.hi[wave] = wdoc1;
+        if (wdoc0 == wdoc1 && !__any(has_row && qdoc < 0)) wdoc = wdoc0;
+        if (lane == 0) docs.lo[wave] = wdoc0, docs.hi[wave] = wdoc1, docs.same[wave] = wave_rows ? wdoc : -3;
         __syncthreads();
         bdoc0 = min(min(docs.lo[0], docs.lo[1]), min(docs.lo[2], docs.lo[3]));
         bdoc1 = max(max(docs.hi[0], docs.hi[1]), max(docs.hi[2], docs.hi[3]));
+        bdoc = docs.same[0];   // the first wave has rows
+#pragma unroll
+        for (int i = 1; i < 4; ++i)
+            if (docs.same[i] != -3 && docs.same[i] != bdoc) bdoc = -2;
         __syncthreads();
     }
     const uint64_t tree = p.tree && has_row ? p.tree[b * (int64_t)p.Sq + qi] : 0;
@@ -170,7 +178,6 @@ __global__ __launch_bounds__(256, 2) void attn_seq_kernel(AttnParams p) {
 
     // this lane's row sees the keys below lim, but for documents and trees
     const int lim = p.causal ? min(len.k, max(pos + 1, prefix)) : len.k;
-    auto in_doc = [&](int j) { return qdoc >= 0 && kdocs[min(j, len.k - 1)] == qdoc; };
     auto in_tree = [&](int j) { return j < len.old || (tree >> ((j - len.old) & 63) & 1); };
 
     // ---- loop ----
@@ -196,10 +203,14 @@ __global__ __launch_bounds__(256, 2) void attn_seq_kernel(AttnParams p) {
         const int j0 = cur.t * kTileKeys, j1 = j0 + kTileKeys - 1;
         // does every row of the block see every key of the tile?
         const bool some = !(j1 < len.k && (!p.causal || j1 <= bpos0 || j1 < prefix) &&
-                            (!kdocs || (cur.same && cur.lo == bdoc0 && bdoc0 == bdoc1)) &&
+                            (!kdocs || (cur.same && cur.lo == bdoc)) &&
                             (!p.tree || j1 < len.old));
         if (some) {
             if (threadIdx.x < 2) bad_keys[stage][threadIdx.x] = 0;
+            if (kdocs && threadIdx.x < kTileKeys) {
+                const int j = j0 + threadIdx.x;
+                tile_docs[stage][threadIdx.x] = j < len.k ? kdocs[j] : -1;
+            }
             __syncthreads();
 #pragma unroll
             for (int i = 0; i < TILE / 8 / 256; ++i) {
@@ -213,7 +224,7 @@ __global__ __launch_bounds__(256, 2) void attn_seq_kernel(AttnParams p) {
                           (!kdocs || (cur.hi >= wdoc0 && cur.lo <= wdoc1));
         if (sees) {
             const bool all = j1 < len.k && (!p.causal || j1 <= wpos0 || j1 < prefix) &&
-                             (!kdocs || (cur.same && cur.lo == wdoc0 && wdoc0 == wdoc1)) &&
+                             (!kdocs || (cur.same && cur.lo == wdoc)) &&
                              (!p.tree || j1 < len.old);
             const uint32_t kt = klds + stage * (TILE * 2), vt = vlds + stage * (TILE * 2);
             f32x16 s[2];
@@ -248,8 +259,17 @@ __global__ __launch_bounds__(256, 2) void attn_seq_kernel(AttnParams p) {
 #pragma unroll
                     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            s[kb][i] = in_doc(j0 + kb * 32 + 8 * (i / 4) + 4 * h + i % 4) ? s[kb][i] : -kInf;
+                        for (int i = 0; i < 4; ++i) {
+                            const int4 d = *reinterpret_cast<const int4*>(&tile_docs[stage][kb * 32 + 8 * i + 4 * h]);
+                            s[kb][4 * i] = d.x == qdoc ? s[kb][4 * i] : -kInf;
+                            s[kb][4 * i + 1] = d.y == qdoc ? s[kb][4 * i + 1] : -kInf;
+                            s[kb][4 * i + 2] = d.z == qdoc ? s[kb][4 * i + 2] : -kInf;
+                            s[kb][4 * i + 3] = d.w == qdoc ? s[kb][4 * i + 3] : -kInf;
+                        }
+                    if (qdoc < 0) {   // of no document
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[0][i] = s[1][i] = -kInf;
+                    }
                 }
                 if (p.tree) {
 #pragma unroll
@@ -279,10 +299,12 @@ __global__ __launch_bounds__(256, 2) void attn_seq_kernel(AttnParams p) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) o[i][e] *= a;
             }
-            // weights, rounded to 16 bits for the second product (to nearest; the
-            // sum takes them unrounded)
+            // weights, rounded to 16 bits for the second product; their sum takes
+            // them as rounded, so that the output is a mean of values, but for parts
+            // whose sums divide fp32 weights later
             u32x4 pf[4];
             const float mb = st.m == -kInf ? 0.0f : st.m;
+            float l2[2] = {st.l, 0.0f};
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -290,16 +312,17 @@ __global__ __launch_bounds__(256, 2) void attn_seq_kernel(AttnParams p) {
                     // a bias may be as low as the type goes, where f x overflows
                     const float w0 = __builtin_amdgcn_exp2f(BIAS ? (s[kb][i] - mb) * f : s[kb][i] * f - st.mf);
                     const float w1 = __builtin_amdgcn_exp2f(BIAS ? (s[kb][i + 1] - mb) * f : s[kb][i + 1] * f - st.mf);
-                    st.l += w0 + w1;
                     pf[kb * 2 + i / 8][i % 8 / 2] = pack2<BF>(w0, w1);
+                    l2[kb] = SPLIT ? l2[kb] + (w0 + w1) : add2<BF>(pf[kb * 2 + i / 8][i % 8 / 2], l2[kb]);
                 }
+            st.l = l2[0] + l2[1];
             weigh_values<D, BF, 4>(o, pf, vt, vfrag);
             if (some) {   // keys with infinities or NaN in their V rows
                 uint64_t bad = (uint64_t)bad_keys[stage][1] << 32 | bad_keys[stage][0];
                 while (bad) {
                     const int j = j0 + __builtin_ctzll(bad);
                     bad &= bad - 1;
-                    const bool mine = has_row && j < lim && (!kdocs || in_doc(j)) && (!p.tree || in_tree(j));
+                    const bool mine = has_row && j < lim && (!kdocs || (qdoc >= 0 && tile_docs[stage][j - j0] == qdoc)) && (!p.tree || in_tree(j));
                     add_values<D, BF>(o, vbase + j * p.vs.r, p.D, h, mine);
                 }
             }

@@ -143,6 +143,15 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
 }
 
+// acc + both of two packed values
+template <bool BF>
+__device__ __forceinline__ float add2(uint32_t v, float acc) {
+    if constexpr (BF)
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, v), bf16x2{(__bf16)1.0f, (__bf16)1.0f}, acc, false);
+    else
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, v), f16x2{(f16)1.0f, (f16)1.0f}, acc, false);
+}
+
 // max / sum with the other half of the wave (lane l ^ 32)
 __device__ __forceinline__ float half_max(float x) {
     const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

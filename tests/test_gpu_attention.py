@@ -144,6 +144,18 @@ def test_documents(pkg, dev, causal, D):
     assert (got[0, 690:] == 0).all()
 
 
+def test_rows_of_no_document(pkg, dev):
+    """Rows without a document among rows that see whole tiles of keys."""
+    import torch
+    q, k, v = _qkv(dev, 1, 200, 320, 2, 1, 64, "f16", seed=16)
+    q_docs = torch.full((1, 200), 3, dtype=torch.int32, device=dev)
+    q_docs[0, [0, 40, 100, 199]] = -1
+    k_docs = torch.full((1, 320), 3, dtype=torch.int32, device=dev)
+    for causal in (False, True):
+        got = _check(pkg, dev, q, k, v, 0.2, q_docs=q_docs, k_docs=k_docs, causal=causal)
+        assert (got[0, [0, 40, 100, 199]] == 0).all()
+
+
 def test_documents_of_other_keys(pkg, dev):
     """Rows and keys with ids of their own, over more than 64 tiles of keys."""
     import torch
