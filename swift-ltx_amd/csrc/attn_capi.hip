@@ -128,7 +128,8 @@ CachedPlan cached_plan(const sltx_kv_cache* c, int tokens, int q_heads, int weig
         splits = std::min<int64_t>({512 / blocks, c->capacity / (4 * kTileKeys), 64});
     }
     p.splits = (int)std::max<int64_t>(1, splits);
-    p.parts = p.splits > 1 || weight_rows > 0;
+    // the kernel of many rows takes a tree (at most 64 tokens) only in parts
+    p.parts = p.splits > 1 || weight_rows > 0 || (!p.few && tokens <= 64);
     if (p.parts) {
         const int64_t dt = c->head_dim > 64 ? 128 : 64;
         p.part_bytes = (size_t)(heads * rows * p.splits) * (size_t)(dt + 2) * sizeof(float);

@@ -85,9 +85,8 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnParams p) {
     f32x16 o[DB];
 #pragma unroll
     for (int i = 0; i < DB; ++i) o[i] = f32x16{};
-    RowState st = {-kInf, 0.0f, 0.0f};
+    RowState<BF> st;
     const float f = CAP ? kLog2e : p.scale * kLog2e;
-    const float grow = 8.0f / f;
     const float yscale = CAP ? p.scale / p.cap : 0.0f;
     const uint32_t kfrag = k_frag_base<D>(lane), vfrag = v_frag_base<D>(lane);
     int stage = 0;
@@ -127,30 +126,8 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnParams p) {
                     s[i] = in_tree(j0 + 8 * (i / 4) + 4 * h + i % 4) ? s[i] : -kInf;
             }
         }
-        float top = s[0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-        top = half_max(top);
-        if (__any(top > st.m + grow)) {
-            const float m = fmaxf(st.m, top);
-            const float mf = m == -kInf ? 0.0f : m * f;
-            const float a = st.m == -kInf ? 0.0f : __builtin_amdgcn_exp2f(st.mf - mf);
-            st.m = m;
-            st.mf = mf;
-            st.l *= a;
-#pragma unroll
-            for (int i = 0; i < DB; ++i)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[i][e] *= a;
-        }
         u32x4 pf[2];
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-            const float w0 = __builtin_amdgcn_exp2f(s[i] * f - st.mf);
-            const float w1 = __builtin_amdgcn_exp2f(s[i + 1] * f - st.mf);
-            st.l += w0 + w1;
-            pf[i / 8][i % 8 / 2] = pack2<BF>(w0, w1);
-        }
+        st.template take<false, SPLIT, DB>(s, f, pf, o);
         weigh_values<D, BF, 2>(o, pf, vt, vfrag);
         while (bad) {
             const int j = j0 + __builtin_ctz(bad);
@@ -175,7 +152,7 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnParams p) {
             for (int i = 0; i < 4; ++i)
                 *reinterpret_cast<f32x4*>(po + 32 * db + 8 * i + 4 * h) =
                     f32x4{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
-        if (h == 0) mls[wave][n][0] = st.m == -kInf ? -kInf : st.mf, mls[wave][n][1] = l;
+        if (h == 0) mls[wave][n][0] = st.mf, mls[wave][n][1] = l;
     }
     __syncthreads();
     for (int e = threadIdx.x; e < rows * (D / 4); e += 256) {
@@ -187,9 +164,9 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnParams p) {
         float lsum = 0.0f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            const float a = mls[w][r][0] == -kInf ? 0.0f : __builtin_amdgcn_exp2f(mls[w][r][0] - m);
+            const float a = __builtin_amdgcn_exp2f(mls[w][r][0] - m);
             lsum += a * mls[w][r][1];
-            // a wave without keys has sums of 0; a weight of 0 must not meet an infinity
+            // a weight of 0 must not meet an infinity
             const f32x4 y = *reinterpret_cast<const f32x4*>(sums + (w * kFewRows + r) * PITCH + c);
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] += a == 0.0f ? 0.0f : a * y[i];
@@ -225,7 +202,7 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(AttnParams p) {
     float l = 0.0f;
     for (int s = lane; s < p.splits; s += 64) {
         const f32x2 x = *reinterpret_cast<const f32x2*>(p.part_ml + (at + (int64_t)s * rows) * 2);
-        if (x[0] != -kInf) l += __builtin_amdgcn_exp2f(x[0] - m) * x[1];
+        l += __builtin_amdgcn_exp2f(x[0] - m) * x[1];
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o, 64);
@@ -233,10 +210,10 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(AttnParams p) {
 #pragma unroll 4
     for (int s = wave; s < p.splits; s += 4) {
         const float ms = p.part_ml[(at + (int64_t)s * rows) * 2];
-        const float a = ms == -kInf ? 0.0f : __builtin_amdgcn_exp2f(ms - m);
+        const float a = __builtin_amdgcn_exp2f(ms - m);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            // a split without keys wrote no sums worth reading
+            // a weight of 0 must not meet an infinity
             const float y = p.part_o[(at + (int64_t)s * rows) * D + i * 64 + lane];
             x[i] += a == 0.0f ? 0.0f : a * y;
         }
@@ -246,7 +223,7 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(AttnParams p) {
     __syncthreads();
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     if (p.row_ml && threadIdx.x == 0)
-        *reinterpret_cast<f32x2*>(p.row_ml + ((int64_t)bh * rows + row) * 2) = f32x2{m == -kInf ? 0.0f : m, inv};
+        *reinterpret_cast<f32x2*>(p.row_ml + ((int64_t)bh * rows + row) * 2) = f32x2{l == 0.0f ? 0.0f : m, inv};
     const int c = threadIdx.x * 2;
     if (c < p.D) {
         const float y0 = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
@@ -313,7 +290,7 @@ __global__ __launch_bounds__(256) void attn_weights_kernel(AttnParams p, float* 
 template <int D, bool BF>
 static hipError_t launch_few(const AttnParams& p, hipStream_t st) {
     const dim3 g(p.B * p.heads * p.splits), t(256);
-    const bool split = p.splits > 1 || p.row_ml;
+    const bool split = p.part_o != nullptr;
     if (p.cap > 0.0f) {
         if (split) hipLaunchKernelGGL((attn_few_kernel<D, BF, kCap | kSplit>), g, t, 0, st, p);
         else hipLaunchKernelGGL((attn_few_kernel<D, BF, kCap>), g, t, 0, st, p);

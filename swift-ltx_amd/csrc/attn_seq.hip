@@ -4,14 +4,15 @@
 //
 // A block of 4 waves takes 128 query rows (32 a wave, Q in registers) over all
 // keys, or over one of `splits` ranges of them.  Tiles of 64 keys pass through
-// two stages of LDS: while one is computed, the copies of the next are in
-// flight.  One pass over the keys with a running maximum and sum; nothing but
+// two stages of LDS, copied while the tiles before are computed.  One pass over the keys with a running maximum and sum; nothing but
 // the output is written.
 #include "attn_tile.hpp"
 
 namespace sltx {
 
-enum : int { kCap = 1, kBias = 2, kSplit = 4 };
+// Variants.  Documents, and the parts that a cached attention is split into (the
+// only ones with a tree), have kernels of their own: their state costs registers.
+enum : int { kCap = 1, kBias = 2, kSplit = 4, kDocs = 8 };
 
 // Documents of a run of 64 tiles (one lane each): the smallest and largest id
 // of a tile's keys, ids below 0 (padding) left out, and whether all are equal.
@@ -21,14 +22,14 @@ struct DocTiles {
 
 template <int D, bool BF, int MODE>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnParams p) {
-    constexpr bool CAP = MODE & kCap, BIAS = MODE & kBias, SPLIT = MODE & kSplit;
+    constexpr bool CAP = MODE & kCap, BIAS = MODE & kBias, SPLIT = MODE & kSplit, DOCS = MODE & kDocs;
     constexpr int TILE = kTileKeys * D;          // values of a tile
     constexpr int QT = D / 16, DB = D / 32;
     constexpr int INSTR = TILE * 2 / 1024 / 4;   // copies of a wave into a tile
     __shared__ __attribute__((aligned(1024))) uint16_t ks[2][TILE], vs[2][TILE];
     __shared__ DocTiles docs;
-    __shared__ __attribute__((aligned(16))) int tile_docs[2][kTileKeys];   // [stage]: documents of the keys
-    __shared__ uint32_t bad_keys[2][2];   // [stage]: keys whose V rows are not finite
+    __shared__ __attribute__((aligned(16))) int tile_docs[kTileKeys];   // documents of a tile's keys
+    __shared__ uint32_t bad_keys[2][2];   // [stage]: its keys whose V rows are not finite
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, h = lane >> 5;
@@ -88,7 +89,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
     // no document)
     int qdoc = -1, wdoc0 = 0x7fffffff, wdoc1 = -1, wdoc = -2, bdoc0 = 0, bdoc1 = 0, bdoc = -2;
     const int32_t* kdocs = nullptr;
-    if (p.q_docs) {
+    if constexpr (DOCS) {
         kdocs = p.k_docs + b * (int64_t)p.Sk;
         qdoc = has_row ? p.q_docs[b * (int64_t)p.Sq + qi] : -1;
         wdoc0 = qdoc >= 0 ? qdoc : 0x7fffffff;
@@ -111,22 +112,22 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
             if (docs.same[i] != -3 && docs.same[i] != bdoc) bdoc = -2;
         __syncthreads();
     }
-    const uint64_t tree = p.tree && has_row ? p.tree[b * (int64_t)p.Sq + qi] : 0;
+    const uint64_t tree = SPLIT && p.tree && has_row ? p.tree[b * (int64_t)p.Sq + qi] : 0;
 
     // ---- copies ----
-    const int kstride = (int)p.ks.r * 2, vstride = (int)p.vs.r * 2, head_bytes = p.D * 2;
-    const uint16_t* kbase = p.k + b * p.ks.b + kvh * p.ks.h;
-    const uint16_t* vbase = p.v + b * p.vs.b + kvh * p.vs.h;
+    const int head_bytes = p.D * 2;
+    const uint16_t* kbase = uniform(p.k + b * p.ks.b + kvh * p.ks.h);
+    const uint16_t* vbase = uniform(p.v + b * p.vs.b + kvh * p.vs.h);
     TileCopy<D, false, INSTR> kc;
     TileCopy<D, true, INSTR> vc;
-    kc.init(wave * INSTR, lane, kstride, head_bytes);
-    vc.init(wave * INSTR, lane, vstride, head_bytes);
+    kc.init(wave * INSTR, lane, (int)p.ks.r * 2, head_bytes);
+    vc.init(wave * INSTR, lane, (int)p.vs.r * 2, head_bytes);
     const uint32_t klds = lds_offset(&ks[0][0]), vlds = lds_offset(&vs[0][0]);
-    auto copy = [&](int t, int stage) {
+    auto copy = [&](int t, int stage) __attribute__((always_inline)) {
         const int64_t j0 = (int64_t)t * kTileKeys;
-        const int rows_left = min(kTileKeys, len.k - (int)j0);
-        const u32x4 kr = tile_rsrc(kbase + j0 * p.ks.r, rows_left, kstride, head_bytes);
-        const u32x4 vr = tile_rsrc(vbase + j0 * p.vs.r, rows_left, vstride, head_bytes);
+        const int left = min(kTileKeys, len.k - (int)j0);
+        const u32x4 kr = tile_rsrc(kbase + j0 * p.ks.r, left, (int)p.ks.r * 2, head_bytes);
+        const u32x4 vr = tile_rsrc(vbase + j0 * p.vs.r, left, (int)p.vs.r * 2, head_bytes);
         const uint32_t at = stage * (TILE * 2) + wave * (INSTR * 1024);
 #pragma unroll
         for (int i = 0; i < INSTR; ++i) copy_1k(kr, kc.off[i], klds + at + i * 1024);
@@ -140,11 +141,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
     // a bit for each.
     uint64_t live = 0;
     int run = first - 64, next_t = first;
-    auto look = [&](int at) {   // all threads: fills docs for tiles at .. at + 63
+    auto look = [&](int at) __attribute__((always_inline)) {   // all threads: fills docs for tiles at .. at + 63
         const int t = threadIdx.x >> 2, j = (at + t) * kTileKeys + (threadIdx.x & 3) * 16;
         int lo = 0x7fffffff, hi = -1, low = 0x7fffffff;
+#pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const int d = j + e < kend ? kdocs[j + e] : -1;
+            const int k = kdocs[min(j + e, kend - 1)], d = j + e < kend ? k : -1;
             lo = min(lo, d < 0 ? 0x7fffffff : d);
             low = min(low, d);
             hi = max(hi, d);
@@ -163,8 +165,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
     struct Tile {
         int t, lo, hi, same;
     };
-    auto advance = [&]() -> Tile {
-        if (!kdocs) return Tile{next_t++, 0, 0, 1};
+    auto advance = [&]() __attribute__((always_inline)) -> Tile {
+        if constexpr (!DOCS) return Tile{next_t++, 0, 0, 1};
         while (live == 0) {
             run += 64;
             if (run >= last) return Tile{last, 0, 0, 0};
@@ -178,157 +180,124 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
 
     // this lane's row sees the keys below lim, but for documents and trees
     const int lim = p.causal ? min(len.k, max(pos + 1, prefix)) : len.k;
-    auto in_tree = [&](int j) { return j < len.old || (tree >> ((j - len.old) & 63) & 1); };
+    auto in_tree = [&](int j) __attribute__((always_inline)) { return j < len.old || (tree >> ((j - len.old) & 63) & 1); };
 
     // ---- loop ----
     f32x16 o[DB];
 #pragma unroll
     for (int i = 0; i < DB; ++i) o[i] = f32x16{};
-    RowState st = {-kInf, 0.0f, 0.0f};
-    const float f = CAP || BIAS ? kLog2e : p.scale * kLog2e;   // exponent = f x
-    const float grow = 8.0f / f;
-    const float yscale = CAP ? p.scale / p.cap : 0.0f;
+    RowState<BF> st;
+    // Weights are exp2(f x).  A capped score is cap tanh(y) = cap - 2 cap t, with
+    // t = 1 / (1 + e^(2 y)): x = -t, the constant drops out of the softmax (with a
+    // bias the score itself is formed).  Off by 9 * 2^-24 cap: enough for weights of
+    // 16 bits.  Parts may serve fp32 weights and take the closer form (capped).
+    const float f = BIAS || (CAP && SPLIT) ? kLog2e : CAP ? 2.0f * p.cap * kLog2e : p.scale * kLog2e;
+    const float capscale = !CAP ? 0.0f : SPLIT ? p.scale / p.cap : 2.0f * kLog2e * p.scale / p.cap;
     const float* bias = BIAS ? p.bias + head * p.bias_h : nullptr;
-    const uint32_t kfrag = k_frag_base<D>(lane), vfrag = v_frag_base<D>(lane);
+    const uint32_t kfrag = klds + k_frag_base<D>(lane), vfrag = vlds + v_frag_base<D>(lane);
 
     Tile cur = advance();
     if (cur.t < last) copy(cur.t, 0);
-    int stage = 0;
-    while (cur.t < last) {
+    for (int stage = 0; cur.t < last; stage ^= 1) {
         const Tile nxt = advance();
-        copies_wait<0>();
-        __syncthreads();     // this tile is in LDS, the other stage free
-        if (nxt.t < last) copy(nxt.t, stage ^ 1);
-
         const int j0 = cur.t * kTileKeys, j1 = j0 + kTileKeys - 1;
         // does every row of the block see every key of the tile?
         const bool some = !(j1 < len.k && (!p.causal || j1 <= bpos0 || j1 < prefix) &&
-                            (!kdocs || (cur.same && cur.lo == bdoc)) &&
-                            (!p.tree || j1 < len.old));
+                            (!DOCS || (cur.same && cur.lo == bdoc)) && (!(SPLIT && p.tree) || j1 < len.old));
+        if (some && threadIdx.x < 2) bad_keys[stage][threadIdx.x] = 0;
+        copies_wait<0>();
+        __syncthreads();     // this tile is in LDS, the other stage free
+        if (nxt.t < last) copy(nxt.t, stage ^ 1);
         if (some) {
-            if (threadIdx.x < 2) bad_keys[stage][threadIdx.x] = 0;
-            if (kdocs && threadIdx.x < kTileKeys) {
-                const int j = j0 + threadIdx.x;
-                tile_docs[stage][threadIdx.x] = j < len.k ? kdocs[j] : -1;
-            }
-            __syncthreads();
 #pragma unroll
             for (int i = 0; i < TILE / 8 / 256; ++i) {
                 const int piece = i * 256 + threadIdx.x, key = piece / (D / 8);
                 if (clear_piece<BF>(vlds + stage * (TILE * 2) + piece * 16))
                     atomicOr(&bad_keys[stage][key >> 5], 1u << (key & 31));
             }
+            if (DOCS && threadIdx.x < kTileKeys) {
+                const int j = j0 + threadIdx.x;
+                tile_docs[threadIdx.x] = j < len.k ? kdocs[j] : -1;
+            }
             __syncthreads();
         }
         const bool sees = wave_rows && (!p.causal || j0 <= wpos1 || j0 < prefix) &&
-                          (!kdocs || (cur.hi >= wdoc0 && cur.lo <= wdoc1));
+                          (!DOCS || (cur.hi >= wdoc0 && cur.lo <= wdoc1));
         if (sees) {
             const bool all = j1 < len.k && (!p.causal || j1 <= wpos0 || j1 < prefix) &&
-                             (!kdocs || (cur.same && cur.lo == wdoc)) &&
-                             (!p.tree || j1 < len.old);
-            const uint32_t kt = klds + stage * (TILE * 2), vt = vlds + stage * (TILE * 2);
+                             (!DOCS || (cur.same && cur.lo == wdoc)) && (!(SPLIT && p.tree) || j1 < len.old);
+            uint32_t ka[QT], va[DB];   // lane addresses of the tile's fragments
+#pragma unroll
+            for (int t = 0; t < QT; ++t) ka[t] = opaque((kfrag ^ (t << 5)) + stage * (TILE * 2));
+#pragma unroll
+            for (int db = 0; db < DB; ++db) va[db] = opaque((vfrag ^ (db << 6)) + stage * (TILE * 2));
             f32x16 s[2];
+            u32x4 pf[2][2];
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
                 s[kb] = f32x16{};
 #pragma unroll
-                for (int t = 0; t < QT; ++t) s[kb] = mfma32<BF>(k_frag<D>(kt, kfrag, kb, t), qf[t], s[kb]);
+                for (int t = 0; t < QT; ++t) s[kb] = mfma32<BF>(lds_16(ka[t] + kb * (64 * D)), qf[t], s[kb]);
             }
-            if constexpr (CAP || BIAS) {
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < 2; ++kb) {
+                if constexpr (CAP || BIAS) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         float x = s[kb][i];
-                        x = CAP ? capped(x * yscale, p.cap) : x * p.scale;
+                        if constexpr (CAP && SPLIT) x = capped(x * capscale, p.cap);
+                        else if constexpr (CAP) x = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(x * capscale));
                         if constexpr (BIAS) {
                             const int j = j0 + kb * 32 + 8 * (i / 4) + 4 * h + i % 4;
-                            x += bias[min(max(j - pos + p.bias_zero, 0), p.bias_n - 1)];
+                            x = (CAP ? p.cap + 2.0f * p.cap * x : x * p.scale) +
+                                bias[min(max(j - pos + p.bias_zero, 0), p.bias_n - 1)];
                         }
                         s[kb][i] = x;
                     }
-            }
-            if (!all) {
-                const int d = lim - j0 - 4 * h;
+                }
+                if (!all) {
+                    const int d = lim - j0 - 4 * h;
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        s[kb][i] = kb * 32 + 8 * (i / 4) + i % 4 < d ? s[kb][i] : -kInf;
-                if (kdocs) {
-#pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
+                    for (int i = 0; i < 16; ++i) s[kb][i] = kb * 32 + 8 * (i / 4) + i % 4 < d ? s[kb][i] : -kInf;
+                    if constexpr (DOCS) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int4 d = *reinterpret_cast<const int4*>(&tile_docs[stage][kb * 32 + 8 * i + 4 * h]);
-                            s[kb][4 * i] = d.x == qdoc ? s[kb][4 * i] : -kInf;
-                            s[kb][4 * i + 1] = d.y == qdoc ? s[kb][4 * i + 1] : -kInf;
-                            s[kb][4 * i + 2] = d.z == qdoc ? s[kb][4 * i + 2] : -kInf;
-                            s[kb][4 * i + 3] = d.w == qdoc ? s[kb][4 * i + 3] : -kInf;
+                            const int4 e = *reinterpret_cast<const int4*>(&tile_docs[kb * 32 + 8 * i + 4 * h]);
+                            s[kb][4 * i] = e.x == qdoc ? s[kb][4 * i] : -kInf;
+                            s[kb][4 * i + 1] = e.y == qdoc ? s[kb][4 * i + 1] : -kInf;
+                            s[kb][4 * i + 2] = e.z == qdoc ? s[kb][4 * i + 2] : -kInf;
+                            s[kb][4 * i + 3] = e.w == qdoc ? s[kb][4 * i + 3] : -kInf;
                         }
-                    if (qdoc < 0) {   // of no document
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) s[0][i] = s[1][i] = -kInf;
+                        if (qdoc < 0) s[kb] = f32x16{} - kInf;   // of no document
                     }
-                }
-                if (p.tree) {
-#pragma unroll
-                    for (int kb = 0; kb < 2; ++kb)
+                    if (SPLIT && p.tree) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
                             s[kb][i] = in_tree(j0 + kb * 32 + 8 * (i / 4) + 4 * h + i % 4) ? s[kb][i] : -kInf;
+                    }
                 }
+                st.template take<BIAS, SPLIT, DB>(s[kb], f, pf[kb], o);
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) {
+                        const uint32_t a = va[db] + (kb * 2 + ks) * (32 * D);
+                        const u32x2 x = lds_tr8(a), y = lds_tr8(a + 16 * D);
+                        o[db] = mfma32<BF>(u32x4{x[0], x[1], y[0], y[1]}, pf[kb][ks], o[db]);
+                    }
             }
-            // the running maximum
-            float top = -kInf;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = fmaxf(top, s[kb][i]);
-            top = half_max(top);
-            if (__any(top > st.m + grow)) {
-                const float m = fmaxf(st.m, top);
-                const float mf = m == -kInf ? 0.0f : m * f;
-                const float a = st.m == -kInf ? 0.0f : BIAS ? __builtin_amdgcn_exp2f((st.m - m) * f)
-                                                            : __builtin_amdgcn_exp2f(st.mf - mf);
-                st.m = m;
-                st.mf = mf;
-                st.l *= a;
-#pragma unroll
-                for (int i = 0; i < DB; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[i][e] *= a;
-            }
-            // weights, rounded to 16 bits for the second product; their sum takes
-            // them as rounded, so that the output is a mean of values, but for parts
-            // whose sums divide fp32 weights later
-            u32x4 pf[4];
-            const float mb = st.m == -kInf ? 0.0f : st.m;
-            float l2[2] = {st.l, 0.0f};
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    // a bias may be as low as the type goes, where f x overflows
-                    const float w0 = __builtin_amdgcn_exp2f(BIAS ? (s[kb][i] - mb) * f : s[kb][i] * f - st.mf);
-                    const float w1 = __builtin_amdgcn_exp2f(BIAS ? (s[kb][i + 1] - mb) * f : s[kb][i + 1] * f - st.mf);
-                    pf[kb * 2 + i / 8][i % 8 / 2] = pack2<BF>(w0, w1);
-                    l2[kb] = SPLIT ? l2[kb] + (w0 + w1) : add2<BF>(pf[kb * 2 + i / 8][i % 8 / 2], l2[kb]);
-                }
-            st.l = l2[0] + l2[1];
-            weigh_values<D, BF, 4>(o, pf, vt, vfrag);
             if (some) {   // keys with infinities or NaN in their V rows
                 uint64_t bad = (uint64_t)bad_keys[stage][1] << 32 | bad_keys[stage][0];
                 while (bad) {
                     const int j = j0 + __builtin_ctzll(bad);
                     bad &= bad - 1;
-                    const bool mine = has_row && j < lim && (!kdocs || (qdoc >= 0 && tile_docs[stage][j - j0] == qdoc)) && (!p.tree || in_tree(j));
+                    const bool mine = has_row && j < lim && (!DOCS || (qdoc >= 0 && tile_docs[j - j0] == qdoc)) &&
+                                      (!(SPLIT && p.tree) || in_tree(j));
                     add_values<D, BF>(o, vbase + j * p.vs.r, p.D, h, mine);
                 }
             }
         }
         cur = nxt;
-        stage ^= 1;
     }
 
     // ---- output ----
@@ -343,7 +312,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
             for (int i = 0; i < 4; ++i)
                 *reinterpret_cast<f32x4*>(po + 32 * db + 8 * i + 4 * h) =
                     f32x4{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
-        if (h == 0) *reinterpret_cast<f32x2*>(p.part_ml + at * 2) = f32x2{st.m == -kInf ? -kInf : st.mf, l};
+        if (h == 0) *reinterpret_cast<f32x2*>(p.part_ml + at * 2) = f32x2{st.mf, l};
     } else {
         // a row that sees nothing is 0
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -360,20 +329,27 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
     }
 }
 
+template <int D, bool BF, int MODE>
+static hipError_t launch_one(const AttnParams& p, dim3 g, hipStream_t st) {
+    hipLaunchKernelGGL((attn_seq_kernel<D, BF, MODE>), g, dim3(256), 0, st, p);
+    return hipGetLastError();
+}
 template <int D, bool BF>
 static hipError_t launch_mode(const AttnParams& p, dim3 g, hipStream_t st) {
-    const int mode = (p.cap > 0.0f ? kCap : 0) | (p.bias ? kBias : 0) | (p.splits > 1 || p.row_ml ? kSplit : 0);
-    const dim3 t(256);
+    const int mode = (p.cap > 0.0f ? kCap : 0) | (p.bias ? kBias : 0) | (p.part_o ? kSplit : 0) | (p.q_docs ? kDocs : 0);
     switch (mode) {
-        case 0: hipLaunchKernelGGL((attn_seq_kernel<D, BF, 0>), g, t, 0, st, p); break;
-        case kCap: hipLaunchKernelGGL((attn_seq_kernel<D, BF, kCap>), g, t, 0, st, p); break;
-        case kBias: hipLaunchKernelGGL((attn_seq_kernel<D, BF, kBias>), g, t, 0, st, p); break;
-        case kCap | kBias: hipLaunchKernelGGL((attn_seq_kernel<D, BF, kCap | kBias>), g, t, 0, st, p); break;
-        case kSplit: hipLaunchKernelGGL((attn_seq_kernel<D, BF, kSplit>), g, t, 0, st, p); break;
-        case kSplit | kCap: hipLaunchKernelGGL((attn_seq_kernel<D, BF, kSplit | kCap>), g, t, 0, st, p); break;
-        default: return hipErrorInvalidValue;   // no caller splits a biased attention
+        case 0: return launch_one<D, BF, 0>(p, g, st);
+        case kCap: return launch_one<D, BF, kCap>(p, g, st);
+        case kBias: return launch_one<D, BF, kBias>(p, g, st);
+        case kCap | kBias: return launch_one<D, BF, kCap | kBias>(p, g, st);
+        case kDocs: return launch_one<D, BF, kDocs>(p, g, st);
+        case kDocs | kCap: return launch_one<D, BF, kDocs | kCap>(p, g, st);
+        case kDocs | kBias: return launch_one<D, BF, kDocs | kBias>(p, g, st);
+        case kDocs | kCap | kBias: return launch_one<D, BF, kDocs | kCap | kBias>(p, g, st);
+        case kSplit: return launch_one<D, BF, kSplit>(p, g, st);
+        case kSplit | kCap: return launch_one<D, BF, kSplit | kCap>(p, g, st);
+        default: return hipErrorInvalidValue;   // parts have neither documents nor a bias
     }
-    return hipGetLastError();
 }
 
 hipError_t launch_attn_seq(AttnParams p, hipStream_t st) {

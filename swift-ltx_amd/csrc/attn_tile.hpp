@@ -90,6 +90,18 @@ __device__ __forceinline__ uint32_t lds_offset(const void* p) {
     return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_char_t)(p));
 }
 
+// A value that the compiler does not take apart again.
+__device__ __forceinline__ uint32_t opaque(uint32_t x) {
+    asm("" : "+v"(x));
+    return x;
+}
+// A pointer that is the same in every lane, held in scalar registers.
+__device__ __forceinline__ const uint16_t* uniform(const uint16_t* p) {
+    const uint64_t a = reinterpret_cast<uint64_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a), hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+    return reinterpret_cast<const uint16_t*>((uint64_t)hi << 32 | lo);
+}
+
 __device__ __forceinline__ u32x4 lds_16(uint32_t a) {
     return *(__attribute__((address_space(3))) const u32x4*)(uintptr_t)(a);
 }
@@ -98,7 +110,8 @@ __device__ __forceinline__ u32x2 lds_tr8(uint32_t a) {
                                          (__attribute__((address_space(3))) s16x4*)(uintptr_t)(a)));
 }
 
-// Lane addresses of the fragments within a tile at LDS offset 0.
+// Lane addresses of the fragments within a tile at LDS offset 0 (or at a multiple
+// of 256 added to the base), and the fragments themselves `tile` bytes further on.
 // K as A operand: lane l holds key l & 31, columns 16 t + 8 (l >> 5) .. + 7.
 template <int D>
 __device__ __forceinline__ uint32_t k_frag_base(int lane) {
@@ -107,7 +120,7 @@ __device__ __forceinline__ uint32_t k_frag_base(int lane) {
 }
 template <int D>
 __device__ __forceinline__ u32x4 k_frag(uint32_t tile, uint32_t base, int block, int t) {
-    return lds_16(tile + block * (64 * D) + (base ^ (t << 5)));
+    return lds_16((base ^ (t << 5)) + tile + block * (64 * D));
 }
 // V^T as A operand of 16 keys: lane l holds column 32 db + (l & 31) and, in the
 // order of P^T's registers, keys 8 (j / 4) + 4 (l >> 5) + j % 4, j = 0..7, of 16:
@@ -119,7 +132,7 @@ __device__ __forceinline__ uint32_t v_frag_base(int lane) {
 }
 template <int D>
 __device__ __forceinline__ u32x4 v_frag(uint32_t tile, uint32_t base, int ks, int db) {
-    const uint32_t a = tile + ks * (32 * D) + (base ^ (db << 6));
+    const uint32_t a = (base ^ (db << 6)) + tile + ks * (32 * D);
     const u32x2 x = lds_tr8(a), y = lds_tr8(a + 16 * D);
     return u32x4{x[0], x[1], y[0], y[1]};
 }
@@ -224,18 +237,91 @@ template <int D, bool BF, int KS>
 __device__ __forceinline__ void weigh_values(f32x16 (&o)[D / 32], const u32x4 (&pf)[KS], uint32_t tile,
                                              uint32_t base) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
+    for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
         for (int db = 0; db < D / 32; ++db) o[db] = mfma32<BF>(v_frag<D>(tile, base, ks, db), pf[ks], o[db]);
+        __builtin_amdgcn_sched_barrier(0);   // few fragments at a time
+    }
 }
 
 // ---- running softmax of one lane's column ----
-// Weights are exp2(f x - mf), with x the (capped, biased) score and mf = f m.  m
-// follows the row's maximum only once that has grown by more than 8 in the
-// exponent: until then weights are at most 2^8, which 16 bits hold as exactly
-// as 1, and no sum has to be rescaled.  m = -inf: nothing seen so far.
+// Weights are exp2(f x - mf), with x the (capped, biased) score.  mf is f times
+// the largest score at some time past, plus kSpare: the row's largest weight
+// then is 2^-kSpare, and as long as no score is kSpare + 1 above it in the
+// exponent, every weight is below 2 and nothing has to be rescaled.  So the
+// weights are formed without a look at the maximum, and one or of their bits
+// tells afterwards whether one reached 2 (or is an infinity or NaN): the top bit
+// of the exponent.  Only then is the maximum taken, and the step done again
+// (grow).  bf16 has range to spare; fp16 keeps 11 binary digits of weights down
+// to 2^-11 of the largest, and 2^-22 of it below.
+template <bool BF>
 struct RowState {
-    float m, mf, l;
+    static constexpr float kSpare = BF ? 7.0f : 3.0f;
+    // Nothing seen so far: finite, so that masked scores (-inf) get the weight 0
+    // and any other an infinite one.
+    static constexpr float kNone = -3.4028235e38f;
+    float m = kNone, mf = kNone, l = 0.0f;
+
+    // p = weights of 32 keys as P^T fragments, rounded to nearest; sum = their sum
+    // as rounded, so that the output is a mean of values, or unrounded where it
+    // will divide fp32 weights (EXACT).  Returns whether a weight of this lane is 2
+    // or more.  BIASED: a bias may be as low as the type goes, where
+    // f x overflows, so the difference is taken first.
+    template <bool BIASED, bool EXACT>
+    __device__ __forceinline__ bool weigh(const f32x16& x, float f, u32x4 (&p)[2], float& sum) const {
+        float a = 0.0f, b = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const float w0 = __builtin_amdgcn_exp2f(BIASED ? (x[i] - m) * f - kSpare : x[i] * f - mf);
+            const float w1 = __builtin_amdgcn_exp2f(BIASED ? (x[i + 1] - m) * f - kSpare : x[i + 1] * f - mf);
+            const uint32_t w = pack2<BF>(w0, w1);
+            p[i / 8][i % 8 / 2] = w;
+            if constexpr (EXACT) i % 4 ? b += w0 + w1 : a += w0 + w1;
+            else i % 4 ? b = add2<BF>(w, b) : a = add2<BF>(w, a);
+        }
+        sum = a + b;
+        uint32_t bits = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) bits |= p[i / 4][i % 4];
+        return (bits & 0x40004000u) != 0;
+    }
+
+    // Keys of a block of 32: their weights, with grow where a lane needs it.
+    template <bool BIASED, bool EXACT, int DB>
+    __device__ __forceinline__ void take(const f32x16& x, float f, u32x4 (&p)[2], f32x16 (&o)[DB]) {
+        float sum;
+        const bool mine = weigh<BIASED, EXACT>(x, f, p, sum);
+        if (__any(mine)) grow<BIASED, EXACT, DB>(mine, x, f, p, sum, o);
+        l += sum;
+    }
+
+    // The same with the maximum taken first, and what was summed so far rescaled,
+    // in the lanes of rows with such a weight: no row's result depends on others.
+    template <bool BIASED, bool EXACT, int DB>
+    __device__ __forceinline__ void grow(bool mine, const f32x16& x, float f, u32x4 (&p)[2], float& sum,
+                                         f32x16 (&o)[DB]) {
+        const auto both = __builtin_amdgcn_permlane32_swap((uint32_t)mine, (uint32_t)mine, false, false);
+        mine = (both[0] | both[1]) != 0;
+        float top = x[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, x[i]);
+        const float old = m;
+        top = half_max(top);
+        m = mine ? fmaxf(m, top) : m;
+        float a = __builtin_amdgcn_exp2f((old - m) * f);
+        if constexpr (!BIASED) {   // exactly what the exponents change by
+            const float mf1 = mine ? m * f + kSpare : mf;
+            a = __builtin_amdgcn_exp2f(mf - mf1);
+            mf = mf1;
+        }
+        asm volatile("" : "+v"(a));   // keeps the products below behind the branch
+        l *= a;
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[i][e] *= a;
+        weigh<BIASED, EXACT>(x, f, p, sum);
+    }
 };
 
 }  // namespace sltx

@@ -6,8 +6,11 @@ of the element type: 2^-11 fp16, 2^-8 bf16):
     of itself, so the sum by u * sum p |v|; an fp16 weight below the normal range
     by 2^-25 of the largest (which is at least 1 before the division);
   * scores are fp32 sums of head_dim products: off by 2^-24 (head_dim + 4) scale
-    sum |q||k| at most, and a few roundings of the score itself (8 * 2^-24 |x|,
-    for a capped one also 4 * 2^-24 cap); a weight follows its exponent's error
+    sum |q||k| at most, and a few roundings of the score itself (8 * 2^-24 |x|);
+    a capped one, cap - 2 cap t with t = 1 / (1 + e^(2 y)), also by what t is off,
+    twice cap times: 2^-23 for the reciprocal's last place, 2^-24 for the sum's
+    rounding, 2^-24 at most for e's (2^-22 of it, t (1 - t) <= 1/4), and by its own
+    rounding: 9 * 2^-24 cap; a weight follows its exponent's error
     e as e^e - 1, on both sides of the division;
   * the output is rounded once more: u of itself (2^-25 below fp16's normal range).
 """
@@ -37,7 +40,7 @@ def head(q, k, v, scale, cap=0.0, bias=None, seen=None):
     slip = 2.0 ** -24 * (q.shape[1] + 4) * mass
     if cap:
         x = cap * torch.tanh(x / cap)
-        slip = slip + 4 * 2.0 ** -24 * cap
+        slip = slip + 9 * 2.0 ** -24 * cap
     if bias is not None:
         x = x + bias.double()
     slip = slip + 8 * 2.0 ** -24 * torch.where(seen, x.abs(), 0.0)
