@@ -38,6 +38,7 @@ struct AttnParams {
     const uint64_t* tree;       // [B, Sq] new tokens that row i sees, or null
     // filled by the launchers
     int pack, heads, tiles, splits;
+    int by_xcd, long_first;     // order of the blocks
     float* part_o;              // [B][heads][splits][Sq * pack][DT] sums of a split
     float* part_ml;             // [B][heads][splits][Sq * pack][2] (f m, l)
     float* row_ml;              // [B][heads][Sq * pack][2] (f m, 1 / l), or null

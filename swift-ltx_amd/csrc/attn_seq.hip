@@ -26,27 +26,39 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
     constexpr int TILE = kTileKeys * D;          // values of a tile
     constexpr int QT = D / 16, DB = D / 32;
     constexpr int INSTR = TILE * 2 / 1024 / 4;   // copies of a wave into a tile
-    __shared__ __attribute__((aligned(1024))) uint16_t ks[2][TILE], vs[2][TILE];
+    // Stages: with three the copies are two tiles ahead, which a block that runs
+    // alone on its CU needs (a tile of 1.05 us waits for memory most of it); at
+    // head_dim 128 a third would leave room for one block on a CU instead of two.
+    constexpr int STAGES = D == 64 ? 3 : 2;
+    __shared__ __attribute__((aligned(1024))) uint16_t ks[STAGES][TILE], vs[STAGES][TILE];
     __shared__ DocTiles docs;
-    __shared__ __attribute__((aligned(16))) int tile_docs[kTileKeys];   // documents of a tile's keys
-    __shared__ uint32_t bad_keys[2][2];   // [stage]: its keys whose V rows are not finite
+    __shared__ __attribute__((aligned(16))) int tile_docs[STAGES][kTileKeys];   // [stage]: documents of a tile's keys
+    __shared__ uint32_t bad_keys[STAGES][2];   // [stage]: its keys whose V rows are not finite
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, h = lane >> 5;
 
-    // Blocks go round the 8 XCDs in turn: each XCD gets a contiguous run of the
-    // (sequence, head, tile, split) order, so that the blocks that share keys
-    // share an L2.  The last tiles, which see the most keys under a causal mask,
-    // come first.
-    const int total = p.B * p.heads * p.tiles * p.splits;
-    const int per = (total + 7) / 8;
-    int w = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if (w >= min(total, ((int)(blockIdx.x & 7) + 1) * per)) return;
-    const int split = SPLIT ? w % p.splits : 0;
-    if (SPLIT) w /= p.splits;
-    const int tile = p.tiles - 1 - w % p.tiles;
-    w /= p.tiles;
-    const int hb = w % p.heads, b = w / p.heads;
+    // Blocks go round the 8 XCDs in turn: each XCD gets a run of the heads (with
+    // their splits), so that the blocks that share keys share an L2.  Under a causal
+    // mask or documents the last tiles of all of the XCD's heads come first: they
+    // see the most keys, and a long one that starts late is waited for at the end.
+    // Else a head's tiles are next to each other.
+    int hs, tile;   // (sequence, head, split), and the tile of rows
+    {
+        const int all = p.B * p.heads * p.splits, each = all / 8;
+        const int i = blockIdx.x >> 3, x = blockIdx.x & 7;
+        if (p.by_xcd) {
+            hs = x * each + (p.long_first ? i % each : i / p.tiles);
+            tile = p.long_first ? i / each : i % p.tiles;
+        } else {
+            hs = blockIdx.x % all;
+            tile = blockIdx.x / all;
+        }
+        tile = p.tiles - 1 - tile;
+    }
+    const int split = SPLIT ? hs % p.splits : 0;
+    if (SPLIT) hs /= p.splits;
+    const int hb = hs % p.heads, b = hs / p.heads;
     const SeqLens len = seq_lens(p, b);
     const int rows = len.q * p.pack;
     const int row0 = tile * kSeqTileRows;
@@ -123,6 +135,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
     kc.init(wave * INSTR, lane, (int)p.ks.r * 2, head_bytes);
     vc.init(wave * INSTR, lane, (int)p.vs.r * 2, head_bytes);
     const uint32_t klds = lds_offset(&ks[0][0]), vlds = lds_offset(&vs[0][0]);
+    const uint32_t dlds = DOCS ? lds_offset(&tile_docs[0][0]) : 0;
     auto copy = [&](int t, int stage) __attribute__((always_inline)) {
         const int64_t j0 = (int64_t)t * kTileKeys;
         const int left = min(kTileKeys, len.k - (int)j0);
@@ -133,13 +146,15 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
         for (int i = 0; i < INSTR; ++i) copy_1k(kr, kc.off[i], klds + at + i * 1024);
 #pragma unroll
         for (int i = 0; i < INSTR; ++i) copy_1k(vr, vc.off[i], vlds + at + i * 1024);
+        if (DOCS && wave == 0)   // keys past the last are masked by it, whatever this gives
+            copy_256(tile_rsrc(reinterpret_cast<const uint16_t*>(kdocs + j0), 1, 0, left * 4), lane * 4, dlds + stage * (kTileKeys * 4));
     };
 
     // ---- which tiles ----
     // The tiles of [first, last) that some row of the block may see, in order.
     // With documents, runs of 64 tiles are looked through at a time: `live` has
     // a bit for each.
-    uint64_t live = 0;
+    uint64_t live = 0, one_b = 0, one_w = 0, seen_w = 0;
     int run = first - 64, next_t = first;
     auto look = [&](int at) __attribute__((always_inline)) {   // all threads: fills docs for tiles at .. at + 63
         const int t = threadIdx.x >> 2, j = (at + t) * kTileKeys + (threadIdx.x & 3) * 16;
@@ -160,22 +175,26 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
         __syncthreads();
         if ((threadIdx.x & 3) == 0) docs.lo[t] = lo, docs.hi[t] = hi, docs.same[t] = low == hi;
         __syncthreads();
-        live = __ballot(at + lane < last && docs.hi[lane] >= bdoc0 && docs.lo[lane] <= bdoc1);
+        const int lo1 = docs.lo[lane], hi1 = docs.hi[lane], one = docs.same[lane] ? lo1 : -4;
+        live = __ballot(at + lane < last && hi1 >= bdoc0 && lo1 <= bdoc1);
+        one_b = __ballot(one == bdoc);
+        one_w = __ballot(one == wdoc);
+        seen_w = __ballot(hi1 >= wdoc0 && lo1 <= wdoc1);
     };
     struct Tile {
-        int t, lo, hi, same;
+        int t;
+        bool one_b, one_w, seen_w;   // of the one document of the block's or the wave's rows; seen by the wave
     };
     auto advance = [&]() __attribute__((always_inline)) -> Tile {
-        if constexpr (!DOCS) return Tile{next_t++, 0, 0, 1};
+        if constexpr (!DOCS) return Tile{next_t++, true, true, true};
         while (live == 0) {
             run += 64;
-            if (run >= last) return Tile{last, 0, 0, 0};
+            if (run >= last) return Tile{last, false, false, false};
             look(run);
         }
         const int i = __builtin_ctzll(live);
         live &= live - 1;
-        return Tile{run + i, __builtin_amdgcn_readfirstlane(docs.lo[i]), __builtin_amdgcn_readfirstlane(docs.hi[i]),
-                    __builtin_amdgcn_readfirstlane(docs.same[i])};
+        return Tile{run + i, (one_b >> i & 1) != 0, (one_w >> i & 1) != 0, (seen_w >> i & 1) != 0};
     };
 
     // this lane's row sees the keys below lim, but for documents and trees
@@ -196,51 +215,67 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
     const float* bias = BIAS ? p.bias + head * p.bias_h : nullptr;
     const uint32_t kfrag = klds + k_frag_base<D>(lane), vfrag = vlds + v_frag_base<D>(lane);
 
-    Tile cur = advance();
-    if (cur.t < last) copy(cur.t, 0);
-    for (int stage = 0; cur.t < last; stage ^= 1) {
-        const Tile nxt = advance();
+    // The tiles are gone through again where that gave an infinity or NaN: then with
+    // care for those in V that only some rows see.
+    for (int careful = 0; careful < 2; ++careful) {
+    bool partly = false;   // some row did not see some key
+    Tile cur = advance(), nxt = cur;
+    if (cur.t < last) {
+        copy(cur.t, 0);
+        nxt = advance();
+        if (STAGES == 3 && nxt.t < last) copy(nxt.t, 1);
+    }
+    for (int stage = 0; cur.t < last; stage = stage + 1 == STAGES ? 0 : stage + 1) {
         const int j0 = cur.t * kTileKeys, j1 = j0 + kTileKeys - 1;
         // does every row of the block see every key of the tile?
         const bool some = !(j1 < len.k && (!p.causal || j1 <= bpos0 || j1 < prefix) &&
-                            (!DOCS || (cur.same && cur.lo == bdoc)) && (!(SPLIT && p.tree) || j1 < len.old));
-        if (some && threadIdx.x < 2) bad_keys[stage][threadIdx.x] = 0;
-        copies_wait<0>();
-        __syncthreads();     // this tile is in LDS, the other stage free
-        if (nxt.t < last) copy(nxt.t, stage ^ 1);
-        if (some) {
+                            cur.one_b && (!(SPLIT && p.tree) || j1 < len.old));
+        partly |= some;
+        if (careful && threadIdx.x < 2) bad_keys[stage][threadIdx.x] = 0;
+        // This tile is in LDS, and the stage of the one before is free.  (A wave of
+        // the first may have a copy of documents more in flight: it waits longer.)
+        if (STAGES == 3 && nxt.t < last) copies_wait<2 * INSTR>();
+        else copies_wait<0>();
+        __syncthreads();
+        Tile far = nxt;
+        if (STAGES == 3 && nxt.t < last) far = advance();
+        if (far.t < last) copy(far.t, stage == 0 ? STAGES - 1 : stage - 1);
+        if (careful && some) {
 #pragma unroll
             for (int i = 0; i < TILE / 8 / 256; ++i) {
                 const int piece = i * 256 + threadIdx.x, key = piece / (D / 8);
                 if (clear_piece<BF>(vlds + stage * (TILE * 2) + piece * 16))
                     atomicOr(&bad_keys[stage][key >> 5], 1u << (key & 31));
             }
-            if (DOCS && threadIdx.x < kTileKeys) {
-                const int j = j0 + threadIdx.x;
-                tile_docs[threadIdx.x] = j < len.k ? kdocs[j] : -1;
-            }
             __syncthreads();
         }
         const bool sees = wave_rows && (!p.causal || j0 <= wpos1 || j0 < prefix) &&
-                          (!DOCS || (cur.hi >= wdoc0 && cur.lo <= wdoc1));
+                          cur.seen_w;
         if (sees) {
             const bool all = j1 < len.k && (!p.causal || j1 <= wpos0 || j1 < prefix) &&
-                             (!DOCS || (cur.same && cur.lo == wdoc)) && (!(SPLIT && p.tree) || j1 < len.old);
+                             cur.one_w && (!(SPLIT && p.tree) || j1 < len.old);
             uint32_t ka[QT], va[DB];   // lane addresses of the tile's fragments
 #pragma unroll
             for (int t = 0; t < QT; ++t) ka[t] = opaque((kfrag ^ (t << 5)) + stage * (TILE * 2));
 #pragma unroll
             for (int db = 0; db < DB; ++db) va[db] = opaque((vfrag ^ (db << 6)) + stage * (TILE * 2));
-            f32x16 s[2];
-            u32x4 pf[2][2];
+            f32x16 s[2] = {};
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                s[kb] = f32x16{};
+            for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                 for (int t = 0; t < QT; ++t) s[kb] = mfma32<BF>(lds_16(ka[t] + kb * (64 * D)), qf[t], s[kb]);
-            }
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
+                u32x4 pf[2], vf[2][DB];
+                // V's fragments are on their way while the weights are formed
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) {
+                        const uint32_t a = va[db] + (kb * 2 + ks) * (32 * D);
+                        const u32x2 x = lds_tr8(a), y = lds_tr8(a + 16 * D);
+                        vf[ks][db] = u32x4{x[0], x[1], y[0], y[1]};
+                    }
                 if constexpr (CAP || BIAS) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
@@ -262,7 +297,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
                     if constexpr (DOCS) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int4 e = *reinterpret_cast<const int4*>(&tile_docs[kb * 32 + 8 * i + 4 * h]);
+                            const int4 e = *reinterpret_cast<const int4*>(&tile_docs[stage][kb * 32 + 8 * i + 4 * h]);
                             s[kb][4 * i] = e.x == qdoc ? s[kb][4 * i] : -kInf;
                             s[kb][4 * i + 1] = e.y == qdoc ? s[kb][4 * i + 1] : -kInf;
                             s[kb][4 * i + 2] = e.z == qdoc ? s[kb][4 * i + 2] : -kInf;
@@ -276,53 +311,66 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
                             s[kb][i] = in_tree(j0 + kb * 32 + 8 * (i / 4) + 4 * h + i % 4) ? s[kb][i] : -kInf;
                     }
                 }
-                st.template take<BIAS, SPLIT, DB>(s[kb], f, pf[kb], o);
+                st.template take<BIAS, SPLIT, DB>(s[kb], f, pf, o);
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-                    for (int db = 0; db < DB; ++db) {
-                        const uint32_t a = va[db] + (kb * 2 + ks) * (32 * D);
-                        const u32x2 x = lds_tr8(a), y = lds_tr8(a + 16 * D);
-                        o[db] = mfma32<BF>(u32x4{x[0], x[1], y[0], y[1]}, pf[kb][ks], o[db]);
-                    }
+                    for (int db = 0; db < DB; ++db) o[db] = mfma32<BF>(vf[ks][db], pf[ks], o[db]);
             }
-            if (some) {   // keys with infinities or NaN in their V rows
+            if (careful && some) {   // keys with infinities or NaN in their V rows
                 uint64_t bad = (uint64_t)bad_keys[stage][1] << 32 | bad_keys[stage][0];
                 while (bad) {
                     const int j = j0 + __builtin_ctzll(bad);
                     bad &= bad - 1;
-                    const bool mine = has_row && j < lim && (!DOCS || (qdoc >= 0 && tile_docs[j - j0] == qdoc)) &&
+                    const bool mine = has_row && j < lim && (!DOCS || (qdoc >= 0 && tile_docs[stage][j - j0] == qdoc)) &&
                                       (!(SPLIT && p.tree) || in_tree(j));
-                    add_values<D, BF>(o, vbase + j * p.vs.r, p.D, h, mine);
+                    const late_params_t e = late_params();
+                    add_values<D, BF>(o, vbase + j * e->vs.r, e->D, h, mine);
                 }
             }
         }
         cur = nxt;
+        nxt = STAGES == 3 || !(nxt.t < last) ? far : advance();
+    }
+    if (careful || !partly) break;
+    float any = 0.0f * st.l;   // NaN where a sum is infinite or NaN
+#pragma unroll
+    for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) any = fmaf(o[i][e], 0.0f, any);
+    if (!__syncthreads_or(has_row && any != any)) break;
+#pragma unroll
+    for (int i = 0; i < DB; ++i) o[i] = f32x16{};
+    st = RowState<BF>();
+    live = 0;
+    run = first - 64;
+    next_t = first;
     }
 
     // ---- output ----
     const float l = half_sum(st.l);
     if (!has_row) return;
+    const late_params_t e = late_params();
     if constexpr (SPLIT) {
-        const int64_t at = ((int64_t)(b * p.heads + hb) * p.splits + split) * ((int64_t)p.Sq * p.pack) + row;
-        float* po = p.part_o + at * D;
+        const int64_t at = ((int64_t)(b * e->heads + hb) * e->splits + split) * ((int64_t)e->Sq * e->pack) + row;
+        float* po = e->part_o + at * D;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 *reinterpret_cast<f32x4*>(po + 32 * db + 8 * i + 4 * h) =
                     f32x4{o[db][4 * i], o[db][4 * i + 1], o[db][4 * i + 2], o[db][4 * i + 3]};
-        if (h == 0) *reinterpret_cast<f32x2*>(p.part_ml + at * 2) = f32x2{st.mf, l};
+        if (h == 0) *reinterpret_cast<f32x2*>(e->part_ml + at * 2) = f32x2{st.mf, l};
     } else {
         // a row that sees nothing is 0
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        uint16_t* out = p.out + b * p.os.b + (int64_t)qi * p.os.r + (int64_t)head * p.os.h;
+        uint16_t* out = e->out + b * e->os.b + (int64_t)qi * e->os.r + (int64_t)head * e->os.h;
 #pragma unroll
         for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int c = 32 * db + 8 * i + 4 * h;
-                if (c < p.D)
+                if (c < e->D)
                     *reinterpret_cast<u32x2*>(out + c) = u32x2{pack2<BF>(o[db][4 * i] * inv, o[db][4 * i + 1] * inv),
                                                               pack2<BF>(o[db][4 * i + 2] * inv, o[db][4 * i + 3] * inv)};
             }
@@ -354,10 +402,12 @@ static hipError_t launch_mode(const AttnParams& p, dim3 g, hipStream_t st) {
 
 hipError_t launch_attn_seq(AttnParams p, hipStream_t st) {
     p.tiles = (int)(((int64_t)p.Sq * p.pack + kSeqTileRows - 1) / kSeqTileRows);
-    const int64_t total = (int64_t)p.B * p.heads * p.tiles * p.splits;
+    const int64_t all = (int64_t)p.B * p.heads * p.splits, total = all * p.tiles;
     if (total == 0) return hipSuccess;
     if (total > 0x7fffff00 / 256) return hipErrorInvalidValue;
-    const dim3 g((unsigned)((total + 7) / 8 * 8));
+    p.by_xcd = all % 8 == 0;
+    p.long_first = p.causal || p.q_docs;
+    const dim3 g((unsigned)total);
     if (p.D > 64) return p.bf16 ? launch_mode<128, true>(p, g, st) : launch_mode<128, false>(p, g, st);
     return p.bf16 ? launch_mode<64, true>(p, g, st) : launch_mode<64, false>(p, g, st);
 }

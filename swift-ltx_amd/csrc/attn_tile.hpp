@@ -82,6 +82,12 @@ __device__ __forceinline__ void copy_1k(u32x4 rsrc, int off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
                  :: "v"(off), "s"(rsrc), "s"(lds) : "memory");
 }
+// The same of 4 bytes a lane.
+__device__ __forceinline__ void copy_256(u32x4 rsrc, int off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dword %0, %1, 0 offen lds"
+                 :: "v"(off), "s"(rsrc), "s"(lds) : "memory");
+}
+// Waits for all but the N copies issued last.
 template <int N>
 __device__ __forceinline__ void copies_wait() {
     asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
@@ -94,6 +100,14 @@ __device__ __forceinline__ uint32_t lds_offset(const void* p) {
 __device__ __forceinline__ uint32_t opaque(uint32_t x) {
     asm("" : "+v"(x));
     return x;
+}
+// A kernel's parameters, loaded where they are used: parameters that only the end
+// or a rare path needs would otherwise be held in scalar registers throughout.
+typedef __attribute__((address_space(4))) const AttnParams* late_params_t;
+__device__ __forceinline__ late_params_t late_params() {
+    auto k = (late_params_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(k));
+    return k;
 }
 // A pointer that is the same in every lane, held in scalar registers.
 __device__ __forceinline__ const uint16_t* uniform(const uint16_t* p) {
