@@ -97,12 +97,93 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendParams p) {
         }
 }
 
+// The same where all of head_dim is rotated in pairs (i, i + D / 2), the usual
+// case: a thread takes the 8 pairs of two pieces, so that each piece is read
+// once, and its loads (two items' at a time) are under way before the angles are
+// there.  750 tokens of 32 + 8 + 8 heads of 128: 5.4 us, 9.2 in the kernel above.
+template <bool BF>
+__global__ __launch_bounds__(256) void kv_append_paired_kernel(AppendParams p) {
+    __shared__ __attribute__((aligned(16))) float cs[kMaxPairs], sn[kMaxPairs];
+    constexpr int AHEAD = 2;
+    const int t = blockIdx.x % p.T, b = blockIdx.x / p.T;
+    const CacheParams& c = p.c;
+    const int half = c.D / 16, qn = p.Hq * half, kn = c.heads * half, items = qn + 2 * kn;
+    const int64_t lb = (int64_t)p.layer * c.B + b;
+    u32x4 lo[AHEAD], hi[AHEAD];
+    auto source = [&](int e) -> const uint16_t* {
+        if (e < qn) return p.q + b * p.qs.b + t * p.qs.r + (e / half) * p.qs.h + e % half * 8;
+        const int i = e - qn;
+        if (i < kn) return p.k + b * p.ks.b + t * p.ks.r + (i / half) * p.ks.h + i % half * 8;
+        return p.v + b * p.vs.b + t * p.vs.r + ((i - kn) / half) * p.vs.h + (i - kn) % half * 8;
+    };
+    auto load = [&](int e0) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int e = e0 + u * 256;
+            if (e < items) {
+                const uint16_t* s = source(e);
+                lo[u] = *reinterpret_cast<const u32x4*>(s);
+                hi[u] = *reinterpret_cast<const u32x4*>(s + c.D / 2);
+            }
+        }
+    };
+    load(threadIdx.x);
+    const int64_t at = (int64_t)c.next[b] + (p.depth ? p.depth[(int64_t)b * p.T + t] : t);
+    const int64_t slot = (int64_t)c.length[b] + t;
+    const bool fits = slot >= 0 && slot < c.capacity;   // tokens past the capacity are dropped
+    if (threadIdx.x < p.pairs) {
+        const double turns = (double)at * (double)p.inv_freq[threadIdx.x] * 0.15915494309189535;
+        sincospif(2.0f * (float)(turns - rint(turns)), &sn[threadIdx.x], &cs[threadIdx.x]);
+    }
+    __syncthreads();
+    for (int e0 = threadIdx.x; e0 < items; e0 += AHEAD * 256) {
+        if (e0 != (int)threadIdx.x) load(e0);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int e = e0 + u * 256;
+            if (e >= items) break;
+            const int i = e < qn ? e : e - qn < kn ? e - qn : e - qn - kn, head = i / half, col = i % half * 8;
+            uint16_t* dst = e < qn ? p.q_out + (((int64_t)b * p.T + t) * p.Hq + head) * c.D
+                                   : (e - qn < kn ? c.k : c.v) + ((lb * c.heads + head) * c.capacity + slot) * c.D;
+            u32x4 x = lo[u], y = hi[u];
+            if (e < qn + kn) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t rx = 0, ry = 0;
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        const float f = widen<BF>(x[w] >> (16 * s) & 0xffffu), g = widen<BF>(y[w] >> (16 * s) & 0xffffu);
+                        const float co = cs[col + 2 * w + s], si = sn[col + 2 * w + s];
+                        rx |= narrow<BF>(f * co - g * si) << (16 * s);
+                        ry |= narrow<BF>(g * co + f * si) << (16 * s);
+                    }
+                    x[w] = rx;
+                    y[w] = ry;
+                }
+            }
+            if (e < qn || fits) {
+                *reinterpret_cast<u32x4*>(dst + col) = x;
+                *reinterpret_cast<u32x4*>(dst + col + c.D / 2) = y;
+            }
+        }
+    }
+    if (c.weight && fits)
+        for (int head = threadIdx.x; head < c.heads; head += 256) {
+            const int64_t i = (lb * c.heads + head) * c.capacity + slot;
+            c.weight[i] = 0.0f;
+            c.position[i] = (int32_t)at;
+        }
+}
+
 hipError_t launch_kv_append(const AppendParams& p, hipStream_t st) {
     const int64_t blocks = (int64_t)p.c.B * p.T;
     if (blocks == 0) return hipSuccess;
     if (blocks > 0x7fffff00 / 256) return hipErrorInvalidValue;
     const dim3 g((unsigned)blocks), t(256);
-    if (p.bf16) hipLaunchKernelGGL(kv_append_kernel<true>, g, t, 0, st, p);
+    if (2 * p.pairs == p.c.D && p.pairs % 8 == 0 && !p.interleaved) {
+        if (p.bf16) hipLaunchKernelGGL(kv_append_paired_kernel<true>, g, t, 0, st, p);
+        else hipLaunchKernelGGL(kv_append_paired_kernel<false>, g, t, 0, st, p);
+    } else if (p.bf16) hipLaunchKernelGGL(kv_append_kernel<true>, g, t, 0, st, p);
     else hipLaunchKernelGGL(kv_append_kernel<false>, g, t, 0, st, p);
     return hipGetLastError();
 }
@@ -207,8 +288,6 @@ hipError_t launch_kv_accept(const CacheParams& c, int drafted, const int32_t* pa
 // four digits of 8 bits, then one pass in slot order for the holes (slots below
 // the budget whose entry goes) and the comers (entries from slots above it that
 // stay), which a second launch moves into them.
-constexpr int kEvictThreads = 1024, kEvictWaves = kEvictThreads / 64;
-
 struct EvictParams {
     CacheParams c;
     int budget, sinks, recent;
@@ -225,10 +304,15 @@ __device__ __forceinline__ uint32_t evict_key(const EvictParams& p, int64_t i, i
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
-__global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictParams p) {
+// A block for each layer, sequence and head.  Wave w takes the slots from w * 64 R
+// on, R at a time in each lane; their keys are read once and kept in registers
+// where R covers them (up to 16384 entries: R = 16 with 16 waves), else (R = 0)
+// read again in each of the seven passes.
+template <int WAVES, int R>
+__global__ __launch_bounds__(WAVES * 64) void kv_evict_select_kernel(EvictParams p) {
     __shared__ int hist[256];
-    __shared__ int sums[kEvictWaves][2];
-    __shared__ int found[2];
+    __shared__ int sums[WAVES][2];
+    __shared__ int found[3];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int lbh = blockIdx.x, b = lbh / p.c.heads % p.c.B;
     const int n = min(p.c.length[b], p.c.capacity);
@@ -237,15 +321,34 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictPar
         return;
     }
     const int64_t after = p.c.next[b], base = (int64_t)lbh * p.c.capacity;
+    const int run = (n + WAVES * 64 - 1) / (WAVES * 64);   // 64 slots each
+    const int s0 = wave * run * 64 + lane;                 // this lane's are s0 + 64 i
+    const int mine = min(run, max(0, (n - s0 + 63) / 64));
+    uint32_t held[R > 0 ? R : 1];
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) held[i] = i < mine ? evict_key(p, base + s0 + i * 64, after) : 0;
+    }
+    // f(slot, key, whether it is one of this lane's), by every lane as often
+    auto each = [&](auto&& f) {
+        if constexpr (R > 0) {
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+                if (i < run) f(s0 + i * 64, held[i], i < mine);
+        } else {
+            for (int i = 0; i < run; ++i)
+                f(s0 + i * 64, i < mine ? evict_key(p, base + s0 + i * 64, after) : 0, i < mine);
+        }
+    };
     uint32_t prefix = 0;
     int want = p.budget;   // of the keys that start with the prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
+    bool exact = false;    // every key that starts with the prefix stays
+    for (int shift = 24; shift >= 0 && !exact; shift -= 8) {
+        for (int i = tid; i < 256; i += WAVES * 64) hist[i] = 0;
         __syncthreads();
-        for (int s = tid; s < n; s += kEvictThreads) {
-            const uint32_t k = evict_key(p, base + s, after);
-            if (shift == 24 || k >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&hist[k >> shift & 255], 1);
-        }
+        each([&](int, uint32_t k, bool in) {
+            if (in && (shift == 24 || k >> (shift + 8) == prefix >> (shift + 8))) atomicAdd(&hist[k >> shift & 255], 1);
+        });
         __syncthreads();
         if (wave == 0) {   // the digit in which the count from the top reaches `want`
             int c[4], sum = 0;
@@ -264,6 +367,7 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictPar
                     if (before < want && before + c[i] >= want) {
                         found[0] = 255 - (lane * 4 + i);
                         found[1] = want - before;
+                        found[2] = before + c[i] == want;
                         break;
                     }
                     before += c[i];
@@ -273,32 +377,33 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictPar
         __syncthreads();
         prefix |= (uint32_t)found[0] << shift;
         want = found[1];
+        exact = found[2] != 0;
         __syncthreads();
     }
-    // `prefix` is the smallest key that stays; `want` of the entries with it do.
-    // Each wave takes a run of slots, a multiple of 64.
-    const int run = (n + kEvictThreads - 1) / kEvictThreads * 64;
-    const int s0 = wave * run, s1 = min(n, s0 + run);
+    // `prefix` is the smallest key that may stay; `want` of the entries with just
+    // it do, the lowest slots, or (exact) every entry from it on.
     const uint64_t below = (1ull << lane) - 1;
-    int ties = 0;
-    for (int s = s0; s < s1; s += 64)
-        ties += __popcll(__ballot(s + lane < s1 && evict_key(p, base + s + lane, after) == prefix));
-    if (lane == 0) sums[wave][0] = ties;
-    __syncthreads();
     int tie0 = 0;
-    for (int w = 0; w < wave; ++w) tie0 += sums[w][0];
-    __syncthreads();
+    if (!exact) {
+        int ties = 0;
+        each([&](int, uint32_t k, bool in) { ties += __popcll(__ballot(in && k == prefix)); });
+        if (lane == 0) sums[wave][0] = ties;
+        __syncthreads();
+        for (int w = 0; w < wave; ++w) tie0 += sums[w][0];
+        __syncthreads();
+    }
     for (int pass = 0; pass < 2; ++pass) {   // count, then write
         int tie = tie0, hole = 0, comer = 0;
         if (pass == 1)
             for (int w = 0; w < wave; ++w) hole += sums[w][0], comer += sums[w][1];
-        for (int s = s0; s < s1; s += 64) {
-            const int slot = s + lane;
-            const uint32_t k = slot < s1 ? evict_key(p, base + slot, after) : 0;
-            const uint64_t t = __ballot(slot < s1 && k == prefix);
-            const bool keep = slot < s1 && (k > prefix || (k == prefix && tie + __popcll(t & below) < want));
-            tie += __popcll(t);
-            const bool is_hole = slot < s1 && slot < p.budget && !keep, is_comer = keep && slot >= p.budget;
+        each([&](int slot, uint32_t k, bool in) {
+            bool keep = in && k >= prefix;
+            if (!exact) {
+                const uint64_t t = __ballot(in && k == prefix);
+                keep = keep && (k > prefix || tie + __popcll(t & below) < want);
+                tie += __popcll(t);
+            }
+            const bool is_hole = in && slot < p.budget && !keep, is_comer = keep && slot >= p.budget;
             const uint64_t hm = __ballot(is_hole), cm = __ballot(is_comer);
             if (pass == 1) {
                 if (is_hole) p.holes[(int64_t)lbh * p.most + hole + __popcll(hm & below)] = slot;
@@ -306,11 +411,11 @@ __global__ __launch_bounds__(kEvictThreads) void kv_evict_select_kernel(EvictPar
             }
             hole += __popcll(hm);
             comer += __popcll(cm);
-        }
+        });
         if (pass == 0) {
             if (lane == 0) sums[wave][0] = hole, sums[wave][1] = comer;
             __syncthreads();
-        } else if (wave == kEvictWaves - 1 && lane == 0) {
+        } else if (wave == WAVES - 1 && lane == 0) {
             p.moves[lbh] = hole;
         }
     }
@@ -353,7 +458,12 @@ hipError_t launch_kv_evict(const CacheParams& c, int budget, int sinks, int rece
     p.moves = static_cast<int32_t*>(ws);
     p.holes = p.moves + lbh;
     p.comers = p.holes + lbh * p.most;
-    hipLaunchKernelGGL(kv_evict_select_kernel, dim3((unsigned)lbh), dim3(kEvictThreads), 0, st, p);
+    // By the capacity: the lengths are on the device.
+    const dim3 g((unsigned)lbh);
+    if (c.capacity <= 256 * 8) hipLaunchKernelGGL((kv_evict_select_kernel<4, 8>), g, dim3(256), 0, st, p);
+    else if (c.capacity <= 1024 * 8) hipLaunchKernelGGL((kv_evict_select_kernel<16, 8>), g, dim3(1024), 0, st, p);
+    else if (c.capacity <= 1024 * 16) hipLaunchKernelGGL((kv_evict_select_kernel<16, 16>), g, dim3(1024), 0, st, p);
+    else hipLaunchKernelGGL((kv_evict_select_kernel<16, 0>), g, dim3(1024), 0, st, p);
     const int64_t pieces = (int64_t)p.most * (c.D / 8);
     const unsigned x = (unsigned)std::max<int64_t>(1, std::min<int64_t>((pieces + 255) / 256, (2048 + lbh - 1) / lbh));
     hipLaunchKernelGGL(kv_evict_move_kernel, dim3(x, (unsigned)lbh), dim3(256), 0, st, p);

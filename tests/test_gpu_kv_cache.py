@@ -296,6 +296,10 @@ EVICT = [  # capacity, lengths, budget, sinks, recent
     (200, [200], 199, 4, 100),
     (128, [128], 1, 0, 1),
     (5000, [4097], 2500, 0, 0),
+    (2048, [2048, 1500], 700, 4, 50),
+    (8192, [8192], 64, 4, 16),
+    (12000, [12000, 9001], 5000, 0, 128),
+    (17000, [17000], 16000, 1, 1),
 ]
 
 
