@@ -114,7 +114,8 @@ int need_workspace(const char* fn, const sltx_kv_cache* c, size_t bytes) {
 struct CachedPlan {
     bool few, parts;
     int splits;
-    size_t part_bytes, bytes;
+    int score_rows, score_pitch;   // scores kept for the weights' sums, or 0
+    size_t part_bytes, row_bytes, bytes;
 };
 CachedPlan cached_plan(const sltx_kv_cache* c, int tokens, int q_heads, int weight_rows) {
     CachedPlan p{};
@@ -133,7 +134,14 @@ CachedPlan cached_plan(const sltx_kv_cache* c, int tokens, int q_heads, int weig
     if (p.parts) {
         const int64_t dt = c->head_dim > 64 ? 128 : 64;
         p.part_bytes = (size_t)(heads * rows * p.splits) * (size_t)(dt + 2) * sizeof(float);
-        p.bytes = p.part_bytes + (size_t)(heads * rows) * 2 * sizeof(float);
+        p.row_bytes = (size_t)(heads * rows + 1) / 2 * 2 * 2 * sizeof(float);   // a multiple of 16
+        p.bytes = p.part_bytes = (p.part_bytes + 15) / 16 * 16;
+        p.bytes += p.row_bytes;
+        if (weight_rows > 0 && weight_rows * pack <= kScoreRows) {
+            p.score_rows = (int)(weight_rows * pack);
+            p.score_pitch = (c->capacity + kFewKeys - 1) / kFewKeys * kFewKeys;
+            p.bytes += (size_t)heads * p.score_rows * p.score_pitch * sizeof(float);
+        }
     }
     return p;
 }
@@ -284,13 +292,20 @@ int sltx_attention_cached(const void* q, const int64_t q_stride[3], const sltx_k
         const int64_t rows = (int64_t)p.B * p.heads * tokens * p.pack;
         p.part_o = static_cast<float*>(cache->workspace);
         p.part_ml = p.part_o + rows * p.splits * (D > 64 ? 128 : 64);
-        if (weight_rows > 0) p.row_ml = reinterpret_cast<float*>(static_cast<char*>(cache->workspace) + plan.part_bytes);
+        char* after = static_cast<char*>(cache->workspace) + plan.part_bytes;
+        if (plan.score_rows > 0) {
+            p.scores = reinterpret_cast<float*>(after + plan.row_bytes);
+            p.score_rows = plan.score_rows;
+            p.score_pitch = plan.score_pitch;
+        } else if (weight_rows > 0) {
+            p.row_ml = reinterpret_cast<float*>(after);
+        }
     }
     hipStream_t st = static_cast<hipStream_t>(stream);
+    float* weight = weight_rows > 0 ? cache->weight + (int64_t)layer * p.B * p.heads * cache->capacity : nullptr;
     hipError_t e = plan.few ? launch_attn_few(p, st) : launch_attn_seq(p, st);
-    if (e == hipSuccess && plan.parts) e = launch_attn_combine(p, st);
-    if (e == hipSuccess && weight_rows > 0)
-        e = launch_attn_weights(p, cache->weight + (int64_t)layer * p.B * p.heads * cache->capacity, weight_rows, st);
+    if (e == hipSuccess && plan.parts) e = launch_attn_finish(p, weight, st);
+    if (e == hipSuccess && p.row_ml) e = launch_attn_weights(p, weight, weight_rows, st);
     return done(e, fn);
 }
 

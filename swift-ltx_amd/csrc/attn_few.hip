@@ -89,13 +89,18 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnParams p) {
     const float f = CAP ? kLog2e : p.scale * kLog2e;
     const float yscale = CAP ? p.scale / p.cap : 0.0f;
     const uint32_t kfrag = k_frag_base<D>(lane), vfrag = v_frag_base<D>(lane);
+    float* score_row = nullptr;
+    if (SPLIT && p.scores && has_row && n < p.score_rows)
+        score_row = p.scores + ((int64_t)bh * p.score_rows + n) * p.score_pitch;
     int stage = 0;
     for (int u = first; u < last; ++u, stage ^= 1) {
         const int j0 = u * kFewKeys + wave * kWaveKeys;
         if (j0 >= len.k) break;   // only in the last unit
         // the next tile's copies may stay in flight
-        if (u + 1 < last && j0 + kFewKeys < len.k) copies_wait<2 * INSTR>();
-        else copies_wait<0>();
+        // (and the 4 stores of the tile before's scores, issued ahead of them)
+        if (!(u + 1 < last && j0 + kFewKeys < len.k)) copies_wait<0>();
+        else if (SPLIT && p.scores && u > first) copies_wait<2 * INSTR + 4>();
+        else copies_wait<2 * INSTR>();
         const uint32_t kt = mine + stage * (2 * TILE * 2), vt = kt + TILE * 2;
         const bool all = j0 + kWaveKeys <= len.old;
         uint32_t bad = 0;   // keys whose V rows are not finite
@@ -125,6 +130,9 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnParams p) {
                 for (int i = 0; i < 16; ++i)
                     s[i] = in_tree(j0 + 8 * (i / 4) + 4 * h + i % 4) ? s[i] : -kInf;
             }
+        }
+        if constexpr (SPLIT) {
+            if (score_row) keep_scores(score_row, j0, h, f, s);
         }
         u32x4 pf[2];
         st.template take<false, SPLIT, DB>(s, f, pf, o);
@@ -185,14 +193,62 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnParams p) {
     }
 }
 
-// One block for each row: out = sum over the splits of exp2(m_s - m) part_s,
-// divided by the same sum of their l.  Four waves take every fourth split.
+// The end of a split attention.  The first blocks take a row each: out = sum over
+// the splits of exp2(m_s - m) part_s, divided by the same sum of their l; four
+// waves take every fourth split.  The others take 1024 keys of a head each, and
+// add the weights of the rows whose scores were kept, exp2(f x - m) / l summed
+// over the rows.
+constexpr int kFinishKeys = 1024;
+
 template <int D, bool BF>
-__global__ __launch_bounds__(256) void attn_combine_kernel(AttnParams p) {
+__global__ __launch_bounds__(256) void attn_finish_kernel(AttnParams p, float* weight) {
     constexpr int PER = D / 64;
     __shared__ float sums[4][D];
+    __shared__ f32x2 ml[kScoreRows];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int rows = p.Sq * p.pack, row = blockIdx.x % rows, bh = blockIdx.x / rows;
+    const int rows = p.Sq * p.pack, outs = p.B * p.heads * rows;
+    if ((int)blockIdx.x >= outs) {
+        const int chunks = (p.Sk + kFinishKeys - 1) / kFinishKeys;
+        const int i = blockIdx.x - outs, bh = i / chunks, j = i % chunks * kFinishKeys + threadIdx.x * 4;
+        const int b = bh / p.heads;
+        const SeqLens len = seq_lens(p, b);
+        if (i % chunks * kFinishKeys >= len.k) return;
+        const float* scores = p.scores + (int64_t)bh * p.score_rows * p.score_pitch + j;
+        {   // 16 lanes for each row
+            const int row = threadIdx.x >> 4, l16 = threadIdx.x & 15;
+            const f32x2* part = reinterpret_cast<const f32x2*>(p.part_ml) + (int64_t)bh * p.splits * rows + min(row, rows - 1);
+            float m = -kInf, l = 0.0f;
+            for (int s = l16; s < p.splits; s += 16) m = fmaxf(m, part[(int64_t)s * rows][0]);
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+            for (int s = l16; s < p.splits; s += 16) {
+                const f32x2 x = part[(int64_t)s * rows];
+                l += __builtin_amdgcn_exp2f(x[0] - m) * x[1];
+            }
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) l += __shfl_xor(l, o, 64);
+            if (l16 == 0) ml[row] = f32x2{m, l == 0.0f ? 0.0f : 1.0f / l};
+        }
+        __syncthreads();
+        if (j >= len.k) return;
+        f32x4 sum = {};
+        for (int r = 0; r < p.score_rows; ++r) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(scores + (int64_t)r * p.score_pitch);
+            const f32x2 c = ml[r];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                // keys before the new tokens are seen by every row
+                const bool sees = j + e < len.old || cached_sees(p, len, b, r / p.pack, j + e);
+                sum[e] += sees ? __builtin_amdgcn_exp2f(x[e] - c[0]) * c[1] : 0.0f;
+            }
+        }
+        float* w = weight + (int64_t)bh * p.Sk + j;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (j + e < len.k) w[e] += sum[e];
+        return;
+    }
+    const int row = blockIdx.x % rows, bh = blockIdx.x / rows;
     const int hb = bh % p.heads, b = bh / p.heads;
     const int64_t at = (int64_t)bh * p.splits * rows + row;   // of split 0
     float m = -kInf;
@@ -234,6 +290,8 @@ __global__ __launch_bounds__(256) void attn_combine_kernel(AttnParams p) {
     }
 }
 
+// The same for more rows, whose scores are formed again (to keep them would write
+// and read 8 bytes for each; reading K again is 2 head_dim for all of them):
 // weight[key] += sum over rows r < wrows of exp2(f x_r - mf_r) / l_r.  S = Q K^T
 // this way round, so that a lane holds 16 rows of one key: the sum over rows is
 // its own.  A wave takes 32 keys; K's fragments come straight from memory.
@@ -274,8 +332,7 @@ __global__ __launch_bounds__(256) void attn_weights_kernel(AttnParams p, float* 
                 const int row = r0 + 8 * (i / 4) + 4 * h + i % 4;
                 if (row < wrows) {
                     const int t = row / p.pack;
-                    const bool sees = j < len.k && (p.tree ? j < len.old || (p.tree[b * (int64_t)p.Sq + t] >> ((j - len.old) & 63) & 1)
-                                                           : j <= len.old + t);
+                    const bool sees = j < len.k && cached_sees(p, len, b, t, j);
                     const float x = CAP ? capped(s[i] * yscale, p.cap) : s[i];
                     const f32x2 ml = *reinterpret_cast<const f32x2*>(row_ml + row * 2);
                     sum += sees ? __builtin_amdgcn_exp2f(x * f - ml[0]) * ml[1] : 0.0f;
@@ -306,14 +363,17 @@ hipError_t launch_attn_few(AttnParams p, hipStream_t st) {
     return p.bf16 ? launch_few<64, true>(p, st) : launch_few<64, false>(p, st);
 }
 
-hipError_t launch_attn_combine(const AttnParams& p, hipStream_t st) {
-    const dim3 g(p.B * p.heads * p.Sq * p.pack), t(256);
+hipError_t launch_attn_finish(const AttnParams& p, float* weight, hipStream_t st) {
+    const int chunks = p.scores ? (p.Sk + kFinishKeys - 1) / kFinishKeys : 0;
+    const int64_t blocks = (int64_t)p.B * p.heads * (p.Sq * p.pack + chunks);
+    if (blocks > 0x7fffff00 / 256) return hipErrorInvalidValue;
+    const dim3 g((unsigned)blocks), t(256);
     if (p.D > 64) {
-        if (p.bf16) hipLaunchKernelGGL((attn_combine_kernel<128, true>), g, t, 0, st, p);
-        else hipLaunchKernelGGL((attn_combine_kernel<128, false>), g, t, 0, st, p);
+        if (p.bf16) hipLaunchKernelGGL((attn_finish_kernel<128, true>), g, t, 0, st, p, weight);
+        else hipLaunchKernelGGL((attn_finish_kernel<128, false>), g, t, 0, st, p, weight);
     } else {
-        if (p.bf16) hipLaunchKernelGGL((attn_combine_kernel<64, true>), g, t, 0, st, p);
-        else hipLaunchKernelGGL((attn_combine_kernel<64, false>), g, t, 0, st, p);
+        if (p.bf16) hipLaunchKernelGGL((attn_finish_kernel<64, true>), g, t, 0, st, p, weight);
+        else hipLaunchKernelGGL((attn_finish_kernel<64, false>), g, t, 0, st, p, weight);
     }
     return hipGetLastError();
 }

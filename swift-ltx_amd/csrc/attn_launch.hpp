@@ -42,6 +42,10 @@ struct AttnParams {
     float* part_o;              // [B][heads][splits][Sq * pack][DT] sums of a split
     float* part_ml;             // [B][heads][splits][Sq * pack][2] (f m, l)
     float* row_ml;              // [B][heads][Sq * pack][2] (f m, 1 / l), or null
+    // f x of the first score_rows rows, -inf where masked, for the weights' sums;
+    // keys of tiles that a row does not see at all may be missing
+    float* scores;              // [B][heads][score_rows][score_pitch], or null
+    int score_rows, score_pitch;
 };
 
 // Keys and rows of sequence b.  Lengths come from device memory: out of range
@@ -68,11 +72,13 @@ constexpr int kFewKeys = 128;       // keys that its four waves take at a time
 
 hipError_t launch_attn_seq(AttnParams p, hipStream_t st);
 hipError_t launch_attn_few(AttnParams p, hipStream_t st);
-// out = sum of the splits' parts, and row_ml where asked for
-hipError_t launch_attn_combine(const AttnParams& p, hipStream_t st);
+// out = sum of the splits' parts; row_ml where asked for; with scores, also
+// weight[b, head, key] += the weights of the first score_rows rows.
+hipError_t launch_attn_finish(const AttnParams& p, float* weight, hipStream_t st);
 // weight[b, head, key] += the weights of the first `rows` query rows, recomputed
 // from row_ml.
 hipError_t launch_attn_weights(const AttnParams& p, float* weight, int rows, hipStream_t st);
+constexpr int kScoreRows = 16;   // most rows whose scores are kept
 
 // ---- cache ----
 struct CacheParams {

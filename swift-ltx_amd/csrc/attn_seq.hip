@@ -197,6 +197,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
         return Tile{run + i, (one_b >> i & 1) != 0, (one_w >> i & 1) != 0, (seen_w >> i & 1) != 0};
     };
 
+    const bool keeps = SPLIT && p.scores && wave_rows && wrow0 < p.score_rows;   // this wave keeps scores
+    float* score_row = nullptr;
+    if (keeps && has_row && row < p.score_rows)
+        score_row = p.scores + ((int64_t)(b * p.heads + hb) * p.score_rows + row) * p.score_pitch;
     // this lane's row sees the keys below lim, but for documents and trees
     const int lim = p.causal ? min(len.k, max(pos + 1, prefix)) : len.k;
     auto in_tree = [&](int j) __attribute__((always_inline)) { return j < len.old || (tree >> ((j - len.old) & 63) & 1); };
@@ -219,6 +223,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
     // care for those in V that only some rows see.
     for (int careful = 0; careful < 2; ++careful) {
     bool partly = false;   // some row did not see some key
+    bool stored = false;   // the wave kept scores of the tile before
     Tile cur = advance(), nxt = cur;
     if (cur.t < last) {
         copy(cur.t, 0);
@@ -234,8 +239,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
         if (careful && threadIdx.x < 2) bad_keys[stage][threadIdx.x] = 0;
         // This tile is in LDS, and the stage of the one before is free.  (A wave of
         // the first may have a copy of documents more in flight: it waits longer.)
+        // The tile before's scores, 8 stores and the last that the wave issued, need not
+        // have arrived.
         if (STAGES == 3 && nxt.t < last) copies_wait<2 * INSTR>();
+        else if (STAGES == 2 && SPLIT && stored) copies_wait<8>();
         else copies_wait<0>();
+        if constexpr (SPLIT) stored = false;
         __syncthreads();
         Tile far = nxt;
         if (STAGES == 3 && nxt.t < last) far = advance();
@@ -252,6 +261,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
         const bool sees = wave_rows && (!p.causal || j0 <= wpos1 || j0 < prefix) &&
                           cur.seen_w;
         if (sees) {
+            if constexpr (SPLIT) stored = keeps;
             const bool all = j1 < len.k && (!p.causal || j1 <= wpos0 || j1 < prefix) &&
                              cur.one_w && (!(SPLIT && p.tree) || j1 < len.old);
             uint32_t ka[QT], va[DB];   // lane addresses of the tile's fragments
@@ -267,15 +277,19 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
                 u32x4 pf[2], vf[2][DB];
-                // V's fragments are on their way while the weights are formed
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks)
+                // V's fragments (at head_dim 128 the first half of them, for registers)
+                // are on their way while the weights are formed
+                constexpr int AHEAD = D == 64 && !SPLIT ? 2 : 1;
+                auto values = [&](int ks) __attribute__((always_inline)) {
 #pragma unroll
                     for (int db = 0; db < DB; ++db) {
                         const uint32_t a = va[db] + (kb * 2 + ks) * (32 * D);
                         const u32x2 x = lds_tr8(a), y = lds_tr8(a + 16 * D);
                         vf[ks][db] = u32x4{x[0], x[1], y[0], y[1]};
                     }
+                };
+#pragma unroll
+                for (int ks = 0; ks < AHEAD; ++ks) values(ks);
                 if constexpr (CAP || BIAS) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
@@ -311,7 +325,12 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
                             s[kb][i] = in_tree(j0 + kb * 32 + 8 * (i / 4) + 4 * h + i % 4) ? s[kb][i] : -kInf;
                     }
                 }
+                if constexpr (SPLIT) {
+                    if (keeps && score_row) keep_scores(score_row, j0 + kb * 32, h, f, s[kb]);
+                }
                 st.template take<BIAS, SPLIT, DB>(s[kb], f, pf, o);
+#pragma unroll
+                for (int ks = AHEAD; ks < 2; ++ks) values(ks);
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks)
 #pragma unroll

@@ -338,4 +338,19 @@ struct RowState {
     }
 };
 
+// Whether new token t sees key j of its sequence.
+__device__ __forceinline__ bool cached_sees(const AttnParams& p, const SeqLens& len, int b, int t, int j) {
+    if (j < len.old) return true;
+    const int u = j - len.old;
+    return p.tree ? (p.tree[b * (int64_t)p.Sq + t] >> (u & 63) & 1) != 0 : u <= t;
+}
+
+// Keeps the scores of 32 keys from j on (those of a lane at 8 (i / 4) + 4 h).
+__device__ __forceinline__ void keep_scores(float* row, int j, int h, float f, const f32x16& x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<f32x4*>(row + j + 8 * i + 4 * h) =
+            f32x4{x[4 * i] * f, x[4 * i + 1] * f, x[4 * i + 2] * f, x[4 * i + 3] * f};
+}
+
 }  // namespace sltx
