@@ -125,8 +125,10 @@ CachedPlan cached_plan(const sltx_kv_cache* c, int tokens, int q_heads, int weig
     if (p.few) {
         splits = std::min<int64_t>({512 / heads, (c->capacity + kFewKeys - 1) / kFewKeys, 256});
     } else {
+        // a tree's rows share blocks of 128 (or 64), in as many ranges of keys as fill
+        // the GPU twice; more tokens only where even blocks of 64 rows leave CUs idle
         const int64_t blocks = heads * ((rows + kSeqTileRows - 1) / kSeqTileRows);
-        splits = std::min<int64_t>({512 / blocks, c->capacity / (4 * kTileKeys), 64});
+        splits = tokens <= 64 || 2 * blocks < kCUs ? std::min<int64_t>({512 / blocks, c->capacity / (4 * kTileKeys), 64}) : 1;
     }
     p.splits = (int)std::max<int64_t>(1, splits);
     // the kernel of many rows takes a tree (at most 64 tokens) only in parts

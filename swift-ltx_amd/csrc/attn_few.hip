@@ -174,10 +174,9 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnParams p) {
         for (int w = 0; w < 4; ++w) {
             const float a = __builtin_amdgcn_exp2f(mls[w][r][0] - m);
             lsum += a * mls[w][r][1];
-            // a weight of 0 must not meet an infinity
             const f32x4 y = *reinterpret_cast<const f32x4*>(sums + (w * kFewRows + r) * PITCH + c);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] += a == 0.0f ? 0.0f : a * y[i];
+            for (int i = 0; i < 4; ++i) x[i] += a * y[i];
         }
         if constexpr (SPLIT) {
             const int64_t at = ((int64_t)bh * p.splits + split) * rows + r;
@@ -269,9 +268,7 @@ __global__ __launch_bounds__(256) void attn_finish_kernel(AttnParams p, float* w
         const float a = __builtin_amdgcn_exp2f(ms - m);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            // a weight of 0 must not meet an infinity
-            const float y = p.part_o[(at + (int64_t)s * rows) * D + i * 64 + lane];
-            x[i] += a == 0.0f ? 0.0f : a * y;
+            x[i] += a * p.part_o[(at + (int64_t)s * rows) * D + i * 64 + lane];
         }
     }
 #pragma unroll

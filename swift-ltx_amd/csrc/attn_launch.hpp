@@ -15,7 +15,7 @@ struct AttnStrides {
     int64_t b, r, h;
 };
 
-// One attention over B sequences; see attn_seq.hip and attn_few.hip.  A block's
+// One attention over B sequences; see attn_seq_kernel.hpp and attn_few.hip.  A block's
 // rows are (query row i, head g of `pack`) pairs, i * pack + g: pack is 1, or
 // the query heads that share a key/value head.
 struct AttnParams {
@@ -39,6 +39,7 @@ struct AttnParams {
     // filled by the launchers
     int pack, heads, tiles, splits;
     int by_xcd, long_first;     // order of the blocks
+    int halves;                 // blocks of 64 rows
     float* part_o;              // [B][heads][splits][Sq * pack][DT] sums of a split
     float* part_ml;             // [B][heads][splits][Sq * pack][2] (f m, l)
     float* row_ml;              // [B][heads][Sq * pack][2] (f m, 1 / l), or null
@@ -65,12 +66,13 @@ __device__ __forceinline__ SeqLens seq_lens(const AttnParams& p, int b) {
     return s;
 }
 
-constexpr int kSeqTileRows = 128;   // query rows of a block of attn_seq.hip
+constexpr int kSeqTileRows = 128;   // query rows of a block of attn_seq_kernel.hpp
 constexpr int kTileKeys = 64;       // keys of its tiles
 constexpr int kFewRows = 32;        // most rows of a block of attn_few.hip
 constexpr int kFewKeys = 128;       // keys that its four waves take at a time
 
 hipError_t launch_attn_seq(AttnParams p, hipStream_t st);
+hipError_t launch_attn_seq_d128(const AttnParams& p, dim3 g, hipStream_t st);
 hipError_t launch_attn_few(AttnParams p, hipStream_t st);
 // out = sum of the splits' parts; row_ml where asked for; with scores, also
 // weight[b, head, key] += the weights of the first score_rows rows.

@@ -1,4 +1,4 @@
-// attn_tile.hpp -- the pieces that the attention kernels share (attn_seq.hip,
+// attn_tile.hpp -- the pieces that the attention kernels share (attn_seq_kernel.hpp,
 // attn_few.hip): tiles of keys and values in LDS, their MFMA fragments, and the
 // softmax's running maximum.
 //
@@ -286,8 +286,9 @@ struct RowState {
         float a = 0.0f, b = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-            const float w0 = __builtin_amdgcn_exp2f(BIASED ? (x[i] - m) * f - kSpare : x[i] * f - mf);
-            const float w1 = __builtin_amdgcn_exp2f(BIASED ? (x[i + 1] - m) * f - kSpare : x[i + 1] * f - mf);
+            // fused by name: the two copies of this (take, grow) have to agree to the bit
+            const float w0 = __builtin_amdgcn_exp2f(BIASED ? fmaf(x[i] - m, f, -kSpare) : fmaf(x[i], f, -mf));
+            const float w1 = __builtin_amdgcn_exp2f(BIASED ? fmaf(x[i + 1] - m, f, -kSpare) : fmaf(x[i + 1], f, -mf));
             const uint32_t w = pack2<BF>(w0, w1);
             p[i / 8][i % 8 / 2] = w;
             if constexpr (EXACT) i % 4 ? b += w0 + w1 : a += w0 + w1;
