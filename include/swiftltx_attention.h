@@ -98,17 +98,18 @@ int sltx_kv_append(const void* q, const int64_t q_stride[3], const void* k, cons
                    int32_t tokens, int32_t q_heads, const float* inv_freq, int32_t pairs,
                    int32_t interleaved, const int32_t* depth, void* q_out, void* stream);
 
-/* Attention of the `tokens` appended tokens over one layer of the cache, q from
- * sltx_kv_append: token t sees the slots below length[b], and of the new tokens
- * those up to t, or with `tree` (uint64 [batch, tokens], tokens <= 64) those u
- * whose bit u is set in tree[b, t] (its ancestors and itself).  x as in
- * sltx_attention, without bias.  out [batch, tokens, q_heads, head_dim] is
+/* Attention of `tokens` of the appended tokens over one layer of the cache, q from
+ * sltx_kv_append: those from the first-th on (0 but where a chunk is taken in more
+ * than one call).  Token t sees the slots below length[b] + first, and of the
+ * tokens of the call those up to t, or with `tree` (uint64 [batch, tokens],
+ * tokens <= 64) those u whose bit u is set in tree[b, t] (its ancestors and
+ * itself).  x as in sltx_attention, without bias.  out [batch, tokens, q_heads, head_dim] is
  * contiguous.  weight_rows > 0 (at most tokens <= 64; the cache has weight)
  * adds to weight the softmax weights of the first weight_rows tokens, summed
  * over the query heads of each key/value head. */
 int sltx_attention_cached(const void* q, const int64_t q_stride[3], const sltx_kv_cache* cache,
-                          int32_t layer, int32_t tokens, int32_t q_heads, float scale, float softcap,
-                          const uint64_t* tree, int32_t weight_rows, void* out, void* stream);
+                          int32_t layer, int32_t first, int32_t tokens, int32_t q_heads, float scale,
+                          float softcap, const uint64_t* tree, int32_t weight_rows, void* out, void* stream);
 /* Bytes of cache->workspace that the call takes, or a negative sltx_status. */
 int64_t sltx_attention_cached_workspace(const sltx_kv_cache* cache, int32_t tokens, int32_t q_heads,
                                         int32_t weight_rows);

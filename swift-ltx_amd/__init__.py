@@ -218,7 +218,7 @@ def lib():
         S = ctypes.POINTER(ctypes.c_int64)
         C = ctypes.POINTER(CKVCache)
         L.sltx_attention.argtypes = [ctypes.POINTER(CAttentionArgs), P]
-        L.sltx_attention_cached.argtypes = [P, S, C, I32, I32, I32, F, F, P, I32, P, P]
+        L.sltx_attention_cached.argtypes = [P, S, C, I32, I32, I32, I32, F, F, P, I32, P, P]
         L.sltx_kv_append.argtypes = [P, S, P, S, P, S, C, I32, I32, I32, P, I32, I32, P, P, P]
         L.sltx_kv_accept.argtypes = [C, I32, P, I32, P, P]
         L.sltx_kv_evict.argtypes = [C, I32, I32, I32, P]
@@ -926,5 +926,5 @@ def load_safetensors(directory):
     return [SafeTensorsFile(os.path.join(directory, f)) for f in names]
 
 
-from .attn import (KVCache, attention, attention_cached, distance_bias, kv_accept,  # noqa: E402
-                   kv_append, kv_evict, rope_inv_freq, tree_masks)
+from .attn import (CachedAttention, KVCache, attention, attention_cached, distance_bias,  # noqa: E402
+                   kv_accept, kv_append, kv_evict, rope_inv_freq, tree_masks)

@@ -228,15 +228,16 @@ class KVCache:
         self.counts.zero_()
 
 
-def attention_cached(q, cache, layer, scale, *, softcap=0.0, tree=None, weight_rows=0, out=None, stream=None):
-    """Attention of the T tokens last appended to `layer` of the cache: q [batch, T,
-    q_heads, head_dim] -> the same shape, contiguous.  Token t sees the sequence's
-    entries and the new tokens up to itself, or with `tree` (int64 [batch, T], T <=
+def attention_cached(q, cache, layer, scale, *, softcap=0.0, tree=None, weight_rows=0, first=0, out=None,
+                     stream=None):
+    """Attention of T of the tokens appended to `layer` of the cache (from the first-th
+    on): q [batch, T, q_heads, head_dim] -> the same shape, contiguous.  Token t sees the sequence's
+    entries, the appended tokens before `first` and those of the call up to itself, or with `tree` (int64 [batch, T], T <=
     64) those whose bit is set in tree[b, t] (tree_masks).  weight_rows: adds the
     attention weights of the first so many tokens to cache.weight (T <= 64)."""
     native = _native()
     if native is not None:
-        r = native.attention_cached(q, *cache._handle, layer, scale, softcap, tree, weight_rows, out, stream)
+        r = native.attention_cached(q, *cache._handle, layer, first, scale, softcap, tree, weight_rows, out, stream)
         if r is not None:
             return r
     import torch
@@ -250,8 +251,8 @@ def attention_cached(q, cache, layer, scale, *, softcap=0.0, tree=None, weight_r
             out = torch.empty(B, T, Hq, D, dtype=q.dtype, device=q.device)
         _need(out, "out", q.shape, (q.dtype,), q.device)
         cache._workspace("sltx_attention_cached_workspace", T, Hq, weight_rows)
-        _P.check(_P.lib().sltx_attention_cached(q.data_ptr(), _strides(q), cache._ref, layer, T, Hq, scale, softcap,
-                                              tree, weight_rows, out.data_ptr(), handle))
+        _P.check(_P.lib().sltx_attention_cached(q.data_ptr(), _strides(q), cache._ref, layer, first, T, Hq, scale,
+                                              softcap, tree, weight_rows, out.data_ptr(), handle))
     return out
 
 
@@ -320,6 +321,59 @@ def kv_evict(cache, budget, *, sinks=4, recent=32, stream=None):
     with _launch(cache.k, stream) as handle:
         cache._workspace("sltx_kv_evict_workspace", budget)
         _P.check(_P.lib().sltx_kv_evict(cache._ref, budget, sinks, recent, handle))
+
+
+class CachedAttention:
+    """What DecodeStep and PrefillStep do between a layer's q|k|v projection and its
+    output projection, over a KVCache of one sequence: rotary embedding, keys and
+    values into the cache, causal attention over it; finish() then counts the tokens
+    (and cuts the cache to `budget` entries).
+
+    config: a ModelConfig (heads, head_dim, rope_theta, rope_scaling).  A cache that
+    tracks weights gets those of each decoded token and of a prompt's last 64.
+    softcap: the cap of the scores (0: none).  sinks, recent: as in kv_evict."""
+
+    WINDOW = 64    # tokens of a prompt whose attention weights count
+
+    def __init__(self, config, cache, stream=None, *, budget=None, sinks=4, recent=32, softcap=0.0):
+        c = config
+        want = (c.num_hidden_layers, 1, c.num_key_value_heads, c.head_dim)
+        if (cache.layers, cache.batch, cache.kv_heads, cache.head_dim) != want:
+            raise ValueError(f"a cache of {want[0]} layers, one sequence, {want[2]} heads of {want[3]} is needed, not "
+                             f"{cache.layers}, {cache.batch}, {cache.kv_heads}, {cache.head_dim}")
+        if cache.dtype != _halves()[0]:
+            raise ValueError(f"the projections are fp16, the cache {cache.dtype}")
+        if budget is not None and cache.weight is None:
+            raise ValueError("a budget needs a cache that tracks weights")
+        self.cache, self.stream, self.softcap = cache, stream, float(softcap)
+        self.heads, self.kv_heads, self.head_dim = c.num_attention_heads, c.num_key_value_heads, c.head_dim
+        self.scale = 1.0 / math.sqrt(c.head_dim)
+        self.inv_freq = rope_inv_freq(c.head_dim, c.rope_theta, c.rope_scaling, device=cache.device)
+        self.budget, self.sinks, self.recent = budget, sinks, recent
+
+    def __call__(self, layer, qkv):
+        """[T, q+k+v] fp16 projections of the next T tokens -> [T, heads * head_dim]."""
+        import torch
+        T, H, K, s = qkv.shape[0], self.heads, self.kv_heads, self.stream
+        x = qkv.view(1, T, H + 2 * K, self.head_dim)
+        q = kv_append(x[:, :, :H], x[:, :, H:H + K], x[:, :, H + K:], self.cache, layer, self.inv_freq, stream=s)
+        cap = self.softcap
+        if self.cache.weight is None or T <= self.WINDOW:
+            rows = 0 if self.cache.weight is None else T
+            out = attention_cached(q, self.cache, layer, self.scale, softcap=cap, weight_rows=rows, stream=s)
+        else:          # the last tokens in a call of their own, which adds their weights
+            n = T - self.WINDOW
+            out = torch.empty_like(q)
+            attention_cached(q[:, :n], self.cache, layer, self.scale, softcap=cap, out=out[:, :n], stream=s)
+            attention_cached(q[:, n:], self.cache, layer, self.scale, softcap=cap, weight_rows=self.WINDOW, first=n,
+                             out=out[:, n:], stream=s)
+        return out.view(T, H * self.head_dim)
+
+    def finish(self, tokens):
+        """After the last layer: the tokens become entries."""
+        kv_accept(self.cache, tokens, stream=self.stream)
+        if self.budget is not None:
+            kv_evict(self.cache, self.budget, sinks=self.sinks, recent=self.recent, stream=self.stream)
 
 
 # ---- what a program prepares once ----

@@ -234,7 +234,7 @@ int64_t sltx_attention_cached_workspace(const sltx_kv_cache* cache, int32_t toke
 }
 
 int sltx_attention_cached(const void* q, const int64_t q_stride[3], const sltx_kv_cache* cache, int32_t layer,
-                          int32_t tokens, int32_t q_heads, float scale, float softcap, const uint64_t* tree,
+                          int32_t first, int32_t tokens, int32_t q_heads, float scale, float softcap, const uint64_t* tree,
                           int32_t weight_rows, void* out, void* stream) {
     const char* fn = "sltx_attention_cached";
     int rc = check_cache(fn, cache);
@@ -242,6 +242,7 @@ int sltx_attention_cached(const void* q, const int64_t q_stride[3], const sltx_k
         (rc = check_heads(fn, cache->dtype, q_heads, cache->kv_heads, cache->head_dim)) != kOk ||
         (rc = check_scores(fn, scale, softcap)) != kOk)
         return rc;
+    if (first < 0 || first > kMaxRows) return set_error(kErrInvalid, "%s: first token %d", fn, first);
     if (tree && tokens > 64) return set_error(kErrInvalid, "%s: a tree of %d tokens (64 at most)", fn, tokens);
     if (weight_rows < 0 || weight_rows > tokens)
         return set_error(kErrInvalid, "%s: weights of %d of %d tokens", fn, weight_rows, tokens);
@@ -286,6 +287,7 @@ int sltx_attention_cached(const void* q, const int64_t q_stride[3], const sltx_k
     p.causal = tree == nullptr;
     p.k_lens = cache->length;
     p.cached = 1;
+    p.first = first;
     p.tree = tree;
     p.pack = q_heads / cache->kv_heads;
     p.heads = cache->kv_heads;

@@ -32,9 +32,10 @@ struct AttnParams {
     const int32_t* prefix;      // [B] keys that every row sees, or null
     const int32_t *q_docs, *k_docs;   // [B, Sq], [B, Sk] or null
     const int32_t *q_lens, *k_lens;   // [B] or null
-    // Over a cache: k_lens are the slots before the new tokens, Sk the capacity,
-    // the keys k_lens[b] + Sq; row i stands at key k_lens[b] + i.
-    int cached;
+    // Over a cache: k_lens + first are the slots before the new tokens, Sk the
+    // capacity, the keys k_lens[b] + first + Sq; row i stands at key k_lens[b] +
+    // first + i.
+    int cached, first;
     const uint64_t* tree;       // [B, Sq] new tokens that row i sees, or null
     // filled by the launchers
     int pack, heads, tiles, splits;
@@ -60,9 +61,9 @@ __device__ __forceinline__ SeqLens seq_lens(const AttnParams& p, int b) {
     SeqLens s;
     s.q = p.q_lens ? min(max(p.q_lens[b], 0), p.Sq) : p.Sq;
     const int k = p.k_lens ? min(max(p.k_lens[b], 0), p.Sk) : p.Sk;
-    s.old = k;
-    s.k = p.cached ? min(k + s.q, p.Sk) : k;
-    s.shift = p.cached ? k : k - s.q;
+    s.old = p.cached ? min(k + p.first, p.Sk) : k;
+    s.k = p.cached ? min(s.old + s.q, p.Sk) : k;
+    s.shift = p.cached ? s.old : k - s.q;
     return s;
 }
 

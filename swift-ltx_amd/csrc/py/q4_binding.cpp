@@ -589,24 +589,24 @@ ENTRY(py_attention) {
     });
 }
 
-// q, cache, device, layer, scale, softcap, tree, weight_rows, out, stream
+// q, cache, device, layer, first, scale, softcap, tree, weight_rows, out, stream
 ENTRY(py_attention_cached) {
-    return guarded(n, 10, [&]() -> PyObject* {
+    return guarded(n, 11, [&]() -> PyObject* {
         int device;
         const sltx_kv_cache* c = cache_of(a[1], a[2], &device);
         const Rows q = rows_of(a[0]);
         need_like(q, c->batch, q.size[1], q.size[2], c->head_dim, cache_type(c), device);
-        const int32_t layer = i32(a[3]), rows = i32(a[7]), T = (int32_t)q.size[1], heads = (int32_t)q.size[2];
-        const float scale = f32(a[4]), cap = f32(a[5]);
-        const auto* tree = static_cast<const uint64_t*>(optional(a[6], at::kLong, device, c->batch, T));
+        const int32_t layer = i32(a[3]), first = i32(a[4]), rows = i32(a[8]), T = (int32_t)q.size[1], heads = (int32_t)q.size[2];
+        const float scale = f32(a[5]), cap = f32(a[6]);
+        const auto* tree = static_cast<const uint64_t*>(optional(a[7], at::kLong, device, c->batch, T));
         const int64_t bytes = f_sltx_attention_cached_workspace(c, T, heads, rows);
         need(bytes >= 0 && (uint64_t)bytes <= c->workspace_bytes);   // else Python grows it
-        void* st = stream_on(a[9], device, a[8] == Py_None);
+        void* st = stream_on(a[10], device, a[9] == Py_None);
         Out out;
-        out.set(a[8], q.size, q.type, tensor(a[0]));
-        if (a[8] != Py_None) need(tensor(a[8]).sizes() == at::IntArrayRef(q.size, 4) && tensor(a[8]).get_device() == device);
+        out.set(a[9], q.size, q.type, tensor(a[0]));
+        if (a[9] != Py_None) need(tensor(a[9]).sizes() == at::IntArrayRef(q.size, 4) && tensor(a[9]).get_device() == device);
         return call([&] {
-                   return f_sltx_attention_cached(q.p, q.stride, c, layer, T, heads, scale, cap, tree, rows, out.ptr, st);
+                   return f_sltx_attention_cached(q.p, q.stride, c, layer, first, T, heads, scale, cap, tree, rows, out.ptr, st);
                }) ? out.give() : nullptr;
     });
 }

@@ -6,11 +6,13 @@ Mirrors LlamaModel.generate / forward / transformerBlock
   embeddingQ4 (Ops.swift:189-208)              sltx_embedding_q4, token id read on the device
   per layer:
     rmsNorm + q, k, v linear                   sltx_rmsnorm_matmul_q4 (q|k|v rows concatenated)
-    rope, KV cache, attention                  the caller's `attention` (outside this library)
+    rope, KV cache, attention                  sltx_kv_append, sltx_attention_cached over `cache`,
+                                               or the caller's `attention`
     o linear                                   sltx_linear
     residualRmsNorm + gate, up, siluMul        sltx_residual_rmsnorm_matmul_q4_silu_mul
     down linear + elemAdd                      sltx_matmul_q4_residual (in place on the residual)
   final rmsNorm + lm_head linear               sltx_rmsnorm_matmul_q4
+  the token's entries count                    sltx_kv_accept (and sltx_kv_evict to a budget)
   argmax / sample                              sltx_argmax / sltx_sample_top_p
 
 The chosen token id stays in device memory and is the next step's input, so a
@@ -21,7 +23,8 @@ with host arguments (seen list, u) runs eagerly.
 
 `attention(layer, qkv)` receives the layer index and the [1, q+k+v] fp16
 projections and returns the [1, heads * head_dim] fp16 attention output (a
-tensor that stays valid until the step ends; a view is fine).  The default is
+tensor that stays valid until the step ends; a view is fine).  With a KVCache
+instead, the step attends over it (CachedAttention).  With neither, it is
 a stand-in with no attention: the q rows themselves, a view of qkv, so the
 data dependency is kept and nothing is launched.
 """
@@ -29,7 +32,7 @@ from __future__ import annotations
 
 import random
 
-from . import (Q4Weight, argmax, embedding_q4, linear, matmul_q4_residual,
+from . import (CachedAttention, Q4Weight, argmax, embedding_q4, linear, matmul_q4_residual,
                rmsnorm_matmul_q4, residual_rmsnorm_matmul_q4_silu_mul, sample, sample_with_state)
 
 
@@ -48,9 +51,13 @@ class DecodeStep:
     layers[i].{qkv_proj, o_proj, gate_proj, up_proj, down_proj,
     input_norm_weight, post_norm_weight}) and a config with hidden_size,
     intermediate_size, num_attention_heads, num_key_value_heads, head_dim,
-    vocab_size, rms_norm_eps."""
+    vocab_size, rms_norm_eps (with a cache also num_hidden_layers, rope_theta,
+    rope_scaling).
 
-    def __init__(self, weights, attention=None, stream=None):
+    cache: a KVCache of one sequence, fp16, which the steps append to; options
+    (budget, sinks, recent, softcap) go to CachedAttention."""
+
+    def __init__(self, weights, attention=None, stream=None, cache=None, **options):
         import torch
         c = weights.config
         self.w = weights
@@ -65,7 +72,10 @@ class DecodeStep:
             for name in ("o_proj", "gate_proj", "up_proj", "down_proj"):
                 if not isinstance(getattr(lw, name), Q4Weight):
                     raise ValueError(f"layer {i}: {name} is not a 4-bit weight")
-        self.attention = attention or q_rows_attention(self.q_dim)
+        if (cache is None and options) or (cache is not None and attention is not None):
+            raise ValueError("either an attention, or a cache and its options")
+        self.cached = None if cache is None else CachedAttention(c, cache, stream, **options)
+        self.attention = self.cached or attention or q_rows_attention(self.q_dim)
         dev = weights.embed_tokens.weight.device
         f16 = torch.float16
         self.token = torch.zeros(1, dtype=torch.int32, device=dev)       # input / chosen token
@@ -95,6 +105,8 @@ class DecodeStep:
         c, w, s = self.c, self.w, self.stream
         embedding_q4(w.embed_tokens, c.vocab_size, self.token, out=self.h, stream=s)
         self._layers()
+        if self.cached is not None:
+            self.cached.finish(1)
         rmsnorm_matmul_q4(self.h, w.norm_weight, c.rms_norm_eps, w.lm_head, c.vocab_size,
                           out=self.logits, stream=s)
 
@@ -125,7 +137,8 @@ class DecodeStep:
         """Capture one step as a HIP graph on self.stream (a torch stream;
         required): greedy, or sampled from `state` (a SamplerState, required
         when temperature > 0).  Runs one eager step there first, which
-        consumes a token, a draw and a history entry like any other step."""
+        consumes a token, a draw, a history entry and a cache entry like any
+        other step."""
         import torch
         if self.stream is None:
             raise ValueError("capture needs a dedicated stream")

@@ -9,7 +9,8 @@ Mirrors LlamaModel.prefill / transformerBlockBatch (LlamaModel.swift:168-203,
     rmsNorm                                     layer 0: sltx_rms_norm (all S rows); later
                                                 layers: the previous down step's call
     q, k, v linear                              sltx_linear, fast (GEMM; q|k|v rows concatenated)
-    RoPE, KV cache append, attention            the caller's `attention` (outside this library)
+    RoPE, KV cache append, attention            sltx_kv_append, sltx_attention_cached over `cache`,
+                                                or the caller's `attention`
     o linear + residualRmsNorm                  sltx_matmul_q4_residual_rms_norm (unrounded sum)
     gate, up linear + siluMul                   sltx_matmul_q4_silu_mul (GEMM, fused epilogue)
     down linear + elemAdd (+ next rmsNorm)      sltx_matmul_q4_residual_rms_norm (rounded sum,
@@ -23,13 +24,15 @@ norm runs on that row alone, fused into the lm_head's GEMV.
 
 `attention(layer, qkv)` receives the layer index and the [S, q+k+v] fp16
 projections and returns the [S, heads * head_dim] fp16 attention output
-(row-contiguous).  The default stand-in has no attention: a copy of the q
+(row-contiguous).  With a KVCache instead, the prompt is appended to it and
+attends over it (CachedAttention): the whole prompt, or the next chunk of one,
+behind the entries that are there.  With neither, the stand-in has no attention: a copy of the q
 columns (torch; it is not part of this path), so every row depends on its own
 token only.
 """
 from __future__ import annotations
 
-from . import (Q4Weight, embedding_q4, linear, matmul_q4_residual, matmul_q4_residual_rms_norm,
+from . import (CachedAttention, Q4Weight, embedding_q4, linear, matmul_q4_residual, matmul_q4_residual_rms_norm,
                matmul_q4_silu_mul, rms_norm, rmsnorm_matmul_q4)
 
 
@@ -44,9 +47,10 @@ class PrefillStep:
     """A prefill over buffers it owns, for prompts of exactly `seq_len` tokens.
 
     weights: a ModelWeights (swiftltx_amd.weights) loaded with concat_qkv, or
-    any object with the same fields (see DecodeStep)."""
+    any object with the same fields (see DecodeStep), and cache and options
+    likewise."""
 
-    def __init__(self, weights, seq_len, attention=None, stream=None):
+    def __init__(self, weights, seq_len, attention=None, stream=None, cache=None, **options):
         import torch
         c = weights.config
         if seq_len < 1:
@@ -64,7 +68,10 @@ class PrefillStep:
             for name in ("o_proj", "gate_proj", "up_proj", "down_proj"):
                 if not isinstance(getattr(lw, name), Q4Weight):
                     raise ValueError(f"layer {i}: {name} is not a 4-bit weight")
-        self.attention = attention or q_columns_attention(self.q_dim)
+        if (cache is None and options) or (cache is not None and attention is not None):
+            raise ValueError("either an attention, or a cache and its options")
+        self.cached = None if cache is None else CachedAttention(c, cache, stream, **options)
+        self.attention = self.cached or attention or q_columns_attention(self.q_dim)
         dev = weights.embed_tokens.weight.device
         f16 = torch.float16
         S, K, F = self.S, self.hidden, c.intermediate_size
@@ -101,6 +108,8 @@ class PrefillStep:
                                             residual_out=self.h, norm_out=self.normed, stream=s)
             else:
                 matmul_q4_residual(self.act, lw.down_proj, self.res, S, K, out=self.h, stream=s)
+        if self.cached is not None:
+            self.cached.finish(S)
         rmsnorm_matmul_q4(self.h[S - 1:], w.norm_weight, eps, w.lm_head, c.vocab_size,
                           out=self.logits, stream=s)
         return self.logits
@@ -108,7 +117,8 @@ class PrefillStep:
     def capture(self):
         """Capture forward() as a HIP graph on self.stream (a torch stream;
         required), after one eager run there (which sizes the workspace the
-        split-K GEMMs and the fused residual + norm calls use in the graph)."""
+        split-K GEMMs and the fused residual + norm calls use in the graph; with
+        a cache it appends the prompt like any other run: reset the cache)."""
         import torch
         if self.stream is None:
             raise ValueError("capture needs a dedicated stream")

@@ -22,8 +22,8 @@ def test_declines_host_tensors_and_wrong_arguments(pkg, native):
     assert native.attention(x, x, x, 1.0, 0.0, None, 0, False, *none[:7]) is None
     assert native.attention(None, x, x, 1.0, 0.0, None, 0, False, *none[:7]) is None
     assert native.attention(x, x) is None
-    assert native.attention_cached(x, *h, 0, 1.0, 0.0, None, 0, None, None) is None
-    assert native.attention_cached(x, 0, 0, 0, 1.0, 0.0, None, 0, None, None) is None
+    assert native.attention_cached(x, *h, 0, 0, 1.0, 0.0, None, 0, None, None) is None
+    assert native.attention_cached(x, 0, 0, 0, 0, 1.0, 0.0, None, 0, None, None) is None
     assert native.kv_append(x, x, x, *h, 0, None, None, False, None, None) is None
     assert native.kv_accept("c", 0, 4, None, None, None) is None
     assert native.kv_evict(*h, 8, 1.0, 2, None) is None

@@ -110,9 +110,10 @@ CACHES = [
 ]
 
 
-def _cached(pkg, c, q=FAR, stride=S3, layer=0, tokens=4, heads=4, scale=0.1, cap=0.0, tree=None, rows=0, out=FAR * 2):
-    return pkg.lib().sltx_attention_cached(q, stride, ctypes.byref(c) if c else None, layer, tokens, heads, scale, cap,
-                                           tree, rows, out, None)
+def _cached(pkg, c, q=FAR, stride=S3, layer=0, tokens=4, heads=4, scale=0.1, cap=0.0, tree=None, rows=0, out=FAR * 2,
+            first=0):
+    return pkg.lib().sltx_attention_cached(q, stride, ctypes.byref(c) if c else None, layer, first, tokens, heads,
+                                           scale, cap, tree, rows, out, None)
 
 
 def _append(pkg, c, q=FAR, k=FAR, v=FAR, stride=S3, layer=0, tokens=4, heads=4, freq=A, pairs=32, depth=None,
@@ -146,6 +147,7 @@ def test_no_cache_and_empty_cache(pkg, call):
     (dict(layer=2), -1, "layer"),
     (dict(layer=-1), -1, "layer"),
     (dict(tokens=-1), -1, "tokens"),
+    (dict(first=-1), -1, "first"),
     (dict(heads=5), -1, "not a multiple"),
     (dict(scale=0.0), -1, "scale"),
     (dict(cap=-1.0), -1, "softcap"),

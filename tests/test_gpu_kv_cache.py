@@ -159,6 +159,32 @@ def test_unused_slots_do_not_matter(pkg, dev, x, T):
                 cache.k[0, b, :, n + T - 1], cache.v[0, b, :, n + T - 1] = old[b]
 
 
+@pytest.mark.parametrize("T,n", [(70, 6), (200, 64), (300, 1)])
+def test_chunk_in_two_calls(pkg, dev, T, n):
+    """The last n of T appended tokens in a call of their own: the same rows as in one
+    call, to the arithmetic's bounds, and their weights."""
+    import torch
+    cache = _cache(pkg, dev, 1, [37, 0], 2, 400, 64, weights=True)
+    q = torch.randn(2, T, 6, 64, device=dev).half()
+    whole = pkg.attention_cached(q, cache, 0, 0.2)
+    before = cache.weight.clone()
+    last = pkg.attention_cached(q[:, T - n:], cache, 0, 0.2, first=T - n, weight_rows=n)
+    early = pkg.attention_cached(q[:, :T - n], cache, 0, 0.2)
+    for b, old in enumerate((37, 0)):
+        want = torch.zeros(2, old + T, dtype=torch.float64, device=dev)
+        j, t = torch.arange(old + T, device=dev)[None] - old, torch.arange(T, device=dev)[:, None]
+        for h in range(6):
+            p, ref, _, bound = R.head(q[b, :, h], cache.k[0, b, h // 3, :old + T], cache.v[0, b, h // 3, :old + T], 0.2,
+                                      0.0, None, j <= t)
+            R.check_out(whole[b, :, h], ref, bound, q.dtype)
+            R.check_out(last[b, :, h], ref[T - n:], bound[T - n:], q.dtype)
+            R.check_out(early[b, :, h], ref[:T - n], bound[:T - n], q.dtype)
+            want[h // 3] += p[T - n:].sum(0)
+        d = (cache.weight[0, b, :, :old + T].double() - before[0, b, :, :old + T].double() - want).abs()
+        assert (d <= 2.0 ** -22 * (1 + want) + 1e-5 * want).all()
+    assert torch.equal(cache.weight[0, 0, :, 37 + T:], before[0, 0, :, 37 + T:])
+
+
 def test_full_cache(pkg, dev):
     """Tokens past the capacity are dropped: not written, not seen, not counted."""
     import torch
