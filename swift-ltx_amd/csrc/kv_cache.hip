@@ -295,13 +295,10 @@ struct EvictParams {
     int most;
 };
 
-__device__ __forceinline__ uint32_t evict_key(const EvictParams& p, int64_t i, int64_t after) {
-    const int32_t at = p.c.position[i];
-    if (at < p.sinks || (int64_t)at >= after - p.recent) return 0xffffffffu;
-    const float w = p.c.weight[i];
-    if (w != w) return 0;
+__device__ __forceinline__ uint32_t evict_key(const EvictParams& p, int32_t at, float w, int64_t after) {
     const uint32_t u = __float_as_uint(w + 0.0f);
-    return u >> 31 ? ~u : u | 0x80000000u;
+    const uint32_t k = w != w ? 0 : u >> 31 ? ~u : u | 0x80000000u;
+    return at < p.sinks || (int64_t)at >= after - p.recent ? 0xffffffffu : k;
 }
 
 // A block for each layer, sequence and head.  Wave w takes the slots from w * 64 R
@@ -325,9 +322,17 @@ __global__ __launch_bounds__(WAVES * 64) void kv_evict_select_kernel(EvictParams
     const int s0 = wave * run * 64 + lane;                 // this lane's are s0 + 64 i
     const int mine = min(run, max(0, (n - s0 + 63) / 64));
     uint32_t held[R > 0 ? R : 1];
-    if constexpr (R > 0) {
+    if constexpr (R > 0) {   // all loads on their way before the first key
+        int32_t at[R];
+        float w[R];
 #pragma unroll
-        for (int i = 0; i < R; ++i) held[i] = i < mine ? evict_key(p, base + s0 + i * 64, after) : 0;
+        for (int i = 0; i < R; ++i) {
+            const int64_t e = base + min(s0 + i * 64, n - 1);
+            at[i] = p.c.position[e];
+            w[i] = p.c.weight[e];
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) held[i] = i < mine ? evict_key(p, at[i], w[i], after) : 0;
     }
     // f(slot, key, whether it is one of this lane's), by every lane as often
     auto each = [&](auto&& f) {
@@ -336,8 +341,10 @@ __global__ __launch_bounds__(WAVES * 64) void kv_evict_select_kernel(EvictParams
             for (int i = 0; i < R; ++i)
                 if (i < run) f(s0 + i * 64, held[i], i < mine);
         } else {
-            for (int i = 0; i < run; ++i)
-                f(s0 + i * 64, i < mine ? evict_key(p, base + s0 + i * 64, after) : 0, i < mine);
+            for (int i = 0; i < run; ++i) {
+                const int64_t e = base + min(s0 + i * 64, n - 1);
+                f(s0 + i * 64, i < mine ? evict_key(p, p.c.position[e], p.c.weight[e], after) : 0, i < mine);
+            }
         }
     };
     uint32_t prefix = 0;

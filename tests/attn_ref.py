@@ -2,9 +2,13 @@
 
 Bounds, element by element, from the arithmetic of the operators (u = half a step
 of the element type: 2^-11 fp16, 2^-8 bf16):
-  * softmax weights are rounded to the type before they meet v: each is off by u
-    of itself, so the sum by u * sum p |v|; an fp16 weight below the normal range
-    by 2^-25 of the largest (which is at least 1 before the division);
+  * softmax weights are rounded to the type before they meet v, and may be summed
+    as they were rounded.  With weights p (1 + d), |d| <= u, in both sums the
+    result is off by sum p d (v - out) / (1 + sum p d), at most
+    u (sum p |v| + |out|) (1 + 2 u);
+  * an fp16 weight below the normal range is off by 2^-25 at most.  Weights are
+    formed against a maximum that may be the row's by up to 2^3 larger, so the
+    largest is at least 2^-3 before the division: 2^-22 of it;
   * scores are fp32 sums of head_dim products: off by 2^-24 (head_dim + 4) scale
     sum |q||k| at most, and a few roundings of the score itself (8 * 2^-24 |x|);
     a capped one, cap - 2 cap t with t = 1 / (1 + e^(2 y)), also by what t is off,
@@ -51,9 +55,9 @@ def head(q, k, v, scale, cap=0.0, bias=None, seen=None):
     weight_bound = torch.expm1(2 * slip) + 4 * 2.0 ** -24
     u = half_step(dt)
     out = p @ v
-    bound = (u + weight_bound) * (p @ v.abs())
+    bound = (u + 2 * u * u + weight_bound) * (p @ v.abs()) + u * (1 + 2 * u) * out.abs()
     if str(dt) == "torch.float16":
-        bound = bound + 2.0 ** -25 * N * (p.amax(1, keepdim=True) * v.abs().amax())
+        bound = bound + 2.0 ** -22 * N * (p.amax(1, keepdim=True) * v.abs().amax())
     return p, out, weight_bound, bound
 
 
