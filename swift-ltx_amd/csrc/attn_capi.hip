@@ -123,7 +123,7 @@ CachedPlan cached_plan(const sltx_kv_cache* c, int tokens, int q_heads, int weig
     p.few = rows <= kFewRows;
     int64_t splits;
     if (p.few) {
-        splits = std::min<int64_t>({512 / heads, (c->capacity + kFewKeys - 1) / kFewKeys, 256});
+        splits = std::min<int64_t>({512 / heads, (c->capacity + kFewKeys - 1) / kFewKeys, kMostSplits});
     } else {
         // a tree's rows share blocks of 128 (or 64), in as many ranges of keys as fill
         // the GPU twice; more tokens only where even blocks of 64 rows leave CUs idle

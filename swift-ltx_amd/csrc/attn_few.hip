@@ -192,12 +192,30 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnParams p) {
     }
 }
 
-// The end of a split attention.  The first blocks take a row each: out = sum over
-// the splits of exp2(m_s - m) part_s, divided by the same sum of their l; four
-// waves take every fourth split.  The others take 1024 keys of a head each, and
-// add the weights of the rows whose scores were kept, exp2(f x - m) / l summed
-// over the rows.
+// The end of a split attention.  A block for each row: out = sum over the splits of
+// exp2(m_s - m) part_s, divided by the same sum of their l; four waves take every
+// fourth split.  Blocks ahead of them take 1024 keys of a head each, and add the
+// weights of the rows whose scores were kept, exp2(f x - m) / l summed over the
+// rows.  What a block reads does not depend on what it computes, so all of it is on
+// its way at once: the launch is one trip to memory long.
 constexpr int kFinishKeys = 1024;
+constexpr int kAhead = 8;   // parts that a wave reads at a time
+
+// (m, l) of a row over all splits, `every` lanes holding every `every`-th split: the
+// lane's own first, in x, then all of them.
+template <int EVERY, int MOST>
+__device__ __forceinline__ f32x2 whole_row(const f32x2 (&x)[MOST / EVERY]) {
+    float m = -kInf, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < MOST / EVERY; ++i) m = fmaxf(m, x[i][0]);
+#pragma unroll
+    for (int o = 1; o < EVERY; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+#pragma unroll
+    for (int i = 0; i < MOST / EVERY; ++i) l += x[i][1] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x[i][0] - m) * x[i][1];
+#pragma unroll
+    for (int o = 1; o < EVERY; o <<= 1) l += __shfl_xor(l, o, 64);
+    return f32x2{m, l};
+}
 
 template <int D, bool BF>
 __global__ __launch_bounds__(256) void attn_finish_kernel(AttnParams p, float* weight) {
@@ -205,70 +223,94 @@ __global__ __launch_bounds__(256) void attn_finish_kernel(AttnParams p, float* w
     __shared__ float sums[4][D];
     __shared__ f32x2 ml[kScoreRows];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int rows = p.Sq * p.pack, outs = p.B * p.heads * rows;
-    if ((int)blockIdx.x >= outs) {
-        const int chunks = (p.Sk + kFinishKeys - 1) / kFinishKeys;
-        const int i = blockIdx.x - outs, bh = i / chunks, j = i % chunks * kFinishKeys + threadIdx.x * 4;
+    const int rows = p.Sq * p.pack;
+    const int chunks = p.scores ? (p.Sk + kFinishKeys - 1) / kFinishKeys : 0;
+    if ((int)blockIdx.x < p.B * p.heads * chunks) {
+        const int bh = blockIdx.x / chunks, j = blockIdx.x % chunks * kFinishKeys + threadIdx.x * 4;
         const int b = bh / p.heads;
-        const SeqLens len = seq_lens(p, b);
-        if (i % chunks * kFinishKeys >= len.k) return;
-        const float* scores = p.scores + (int64_t)bh * p.score_rows * p.score_pitch + j;
-        {   // 16 lanes for each row
-            const int row = threadIdx.x >> 4, l16 = threadIdx.x & 15;
-            const f32x2* part = reinterpret_cast<const f32x2*>(p.part_ml) + (int64_t)bh * p.splits * rows + min(row, rows - 1);
-            float m = -kInf, l = 0.0f;
-            for (int s = l16; s < p.splits; s += 16) m = fmaxf(m, part[(int64_t)s * rows][0]);
+        // the (m, l) of the rows: 16 lanes for each
+        const int row = threadIdx.x >> 4, l16 = threadIdx.x & 15;
+        const f32x2* part = reinterpret_cast<const f32x2*>(p.part_ml) + (int64_t)bh * p.splits * rows + min(row, rows - 1);
+        f32x2 parts[kMostSplits / 16];
 #pragma unroll
-            for (int o = 1; o < 16; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-            for (int s = l16; s < p.splits; s += 16) {
-                const f32x2 x = part[(int64_t)s * rows];
-                l += __builtin_amdgcn_exp2f(x[0] - m) * x[1];
-            }
-#pragma unroll
-            for (int o = 1; o < 16; o <<= 1) l += __shfl_xor(l, o, 64);
-            if (l16 == 0) ml[row] = f32x2{m, l == 0.0f ? 0.0f : 1.0f / l};
+        for (int i = 0; i < kMostSplits / 16; ++i) {
+            parts[i] = f32x2{-kInf, 0.0f};
+            if (i * 16 < p.splits && i * 16 + l16 < p.splits) parts[i] = part[(int64_t)(i * 16 + l16) * rows];
         }
+        const SeqLens len = seq_lens(p, b);
+        if (blockIdx.x % chunks * kFinishKeys >= len.k) return;
+        const float* scores = p.scores + (int64_t)bh * p.score_rows * p.score_pitch + j;
+        float* w = weight + (int64_t)bh * p.Sk + j;
+        f32x4 x[4], sum = {};
+        auto read = [&](int r0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (r0 + i < p.score_rows && j < len.k)
+                    x[i] = *reinterpret_cast<const f32x4*>(scores + (int64_t)(r0 + i) * p.score_pitch);
+        };
+        read(0);
+        float old[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) old[e] = j + e < len.k ? w[e] : 0.0f;
+        const f32x2 r = whole_row<16, kMostSplits>(parts);
+        if (l16 == 0) ml[row] = f32x2{r[0], r[1] == 0.0f ? 0.0f : 1.0f / r[1]};
         __syncthreads();
         if (j >= len.k) return;
-        f32x4 sum = {};
-        for (int r = 0; r < p.score_rows; ++r) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(scores + (int64_t)r * p.score_pitch);
-            const f32x2 c = ml[r];
+        for (int r0 = 0; r0 < p.score_rows; r0 += 4) {
+            if (r0 > 0) read(r0);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                // keys before the new tokens are seen by every row
-                const bool sees = j + e < len.old || cached_sees(p, len, b, r / p.pack, j + e);
-                sum[e] += sees ? __builtin_amdgcn_exp2f(x[e] - c[0]) * c[1] : 0.0f;
+            for (int i = 0; i < 4; ++i) {
+                if (r0 + i >= p.score_rows) break;
+                const f32x2 c = ml[r0 + i];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    // keys before the new tokens are seen by every row
+                    const bool sees = j + e < len.old || cached_sees(p, len, b, (r0 + i) / p.pack, j + e);
+                    sum[e] += sees ? __builtin_amdgcn_exp2f(x[i][e] - c[0]) * c[1] : 0.0f;
+                }
             }
         }
-        float* w = weight + (int64_t)bh * p.Sk + j;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (j + e < len.k) w[e] += sum[e];
+            if (j + e < len.k) w[e] = old[e] + sum[e];
         return;
     }
-    const int row = blockIdx.x % rows, bh = blockIdx.x / rows;
+    const int block = blockIdx.x - p.B * p.heads * chunks;
+    const int row = block % rows, bh = block / rows;
     const int hb = bh % p.heads, b = bh / p.heads;
     const int64_t at = (int64_t)bh * p.splits * rows + row;   // of split 0
-    float m = -kInf;
-    for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, p.part_ml[(at + (int64_t)s * rows) * 2]);
+    const f32x2* part_ml = reinterpret_cast<const f32x2*>(p.part_ml) + at;
+    const float* part_o = p.part_o + at * D + lane;
+    f32x2 parts[kMostSplits / 64];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    float l = 0.0f;
-    for (int s = lane; s < p.splits; s += 64) {
-        const f32x2 x = *reinterpret_cast<const f32x2*>(p.part_ml + (at + (int64_t)s * rows) * 2);
-        l += __builtin_amdgcn_exp2f(x[0] - m) * x[1];
+    for (int i = 0; i < kMostSplits / 64; ++i) {
+        parts[i] = f32x2{-kInf, 0.0f};
+        if (i * 64 < p.splits && i * 64 + lane < p.splits) parts[i] = part_ml[(int64_t)(i * 64 + lane) * rows];
     }
+    // kAhead of the wave's parts, and their m
+    float y[kAhead][PER], ms[kAhead];
+    auto read = [&](int s0) {
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o, 64);
+        for (int i = 0; i < kAhead; ++i) {
+            const int s = s0 + 4 * i;
+            if (s >= p.splits) break;
+            ms[i] = part_ml[(int64_t)s * rows][0];
+#pragma unroll
+            for (int c = 0; c < PER; ++c) y[i][c] = part_o[(int64_t)s * rows * D + c * 64];
+        }
+    };
+    read(wave);
+    const f32x2 whole = whole_row<64, kMostSplits>(parts);
+    const float m = whole[0], l = whole[1];
     float x[PER] = {};
-#pragma unroll 4
-    for (int s = wave; s < p.splits; s += 4) {
-        const float ms = p.part_ml[(at + (int64_t)s * rows) * 2];
-        const float a = __builtin_amdgcn_exp2f(ms - m);
+    for (int s0 = wave; s0 < p.splits; s0 += 4 * kAhead) {
+        if (s0 > wave) read(s0);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            x[i] += a * p.part_o[(at + (int64_t)s * rows) * D + i * 64 + lane];
+        for (int i = 0; i < kAhead; ++i) {
+            if (s0 + 4 * i >= p.splits) break;
+            const float a = __builtin_amdgcn_exp2f(ms[i] - m);
+#pragma unroll
+            for (int c = 0; c < PER; ++c) x[c] += a * y[i][c];
         }
     }
 #pragma unroll

@@ -81,6 +81,7 @@ hipError_t launch_attn_finish(const AttnParams& p, float* weight, hipStream_t st
 // weight[b, head, key] += the weights of the first `rows` query rows, recomputed
 // from row_ml.
 hipError_t launch_attn_weights(const AttnParams& p, float* weight, int rows, hipStream_t st);
+constexpr int kMostSplits = 256;   // ranges of keys that an attention is split into
 constexpr int kScoreRows = 16;   // most rows whose scores are kept
 
 // ---- cache ----
