@@ -115,7 +115,7 @@ struct CachedPlan {
     bool few, parts;
     int splits;
     int score_rows, score_pitch;   // scores kept for the weights' sums, or 0
-    size_t part_bytes, row_bytes, bytes;
+    size_t part_bytes, row_bytes, shares, score, bytes;   // shares, score: where they start
 };
 CachedPlan cached_plan(const sltx_kv_cache* c, int tokens, int q_heads, int weight_rows) {
     CachedPlan p{};
@@ -123,7 +123,7 @@ CachedPlan cached_plan(const sltx_kv_cache* c, int tokens, int q_heads, int weig
     p.few = rows <= kFewRows;
     int64_t splits;
     if (p.few) {
-        splits = std::min<int64_t>({512 / heads, (c->capacity + kFewKeys - 1) / kFewKeys, kMostSplits});
+        splits = std::min<int64_t>({(c->head_dim > 64 ? 256 : 512) / heads, (c->capacity + kFewKeys - 1) / kFewKeys, kMostSplits});
     } else {
         // a tree's rows share blocks of 128 (or 64), in as many ranges of keys as fill
         // the GPU twice; more tokens only where even blocks of 64 rows leave CUs idle
@@ -139,6 +139,9 @@ CachedPlan cached_plan(const sltx_kv_cache* c, int tokens, int q_heads, int weig
         p.row_bytes = (size_t)(heads * rows + 1) / 2 * 2 * 2 * sizeof(float);   // a multiple of 16
         p.bytes = p.part_bytes = (p.part_bytes + 15) / 16 * 16;
         p.bytes += p.row_bytes;
+        p.shares = p.bytes;
+        p.bytes += ((size_t)c->batch * 2 * sizeof(int32_t) + 15) / 16 * 16;
+        p.score = p.bytes;
         if (weight_rows > 0 && weight_rows * pack <= kScoreRows) {
             p.score_rows = (int)(weight_rows * pack);
             p.score_pitch = (c->capacity + kFewKeys - 1) / kFewKeys * kFewKeys;
@@ -292,13 +295,15 @@ int sltx_attention_cached(const void* q, const int64_t q_stride[3], const sltx_k
     p.pack = q_heads / cache->kv_heads;
     p.heads = cache->kv_heads;
     p.splits = plan.splits;
+    p.unit_bits = __builtin_ctz(plan.few ? kFewKeys : kTileKeys);
     if (plan.parts) {
         const int64_t rows = (int64_t)p.B * p.heads * tokens * p.pack;
         p.part_o = static_cast<float*>(cache->workspace);
         p.part_ml = p.part_o + rows * p.splits * (D > 64 ? 128 : 64);
         char* after = static_cast<char*>(cache->workspace) + plan.part_bytes;
+        p.shares = reinterpret_cast<int32_t*>(static_cast<char*>(cache->workspace) + plan.shares);
         if (plan.score_rows > 0) {
-            p.scores = reinterpret_cast<float*>(after + plan.row_bytes);
+            p.scores = reinterpret_cast<float*>(static_cast<char*>(cache->workspace) + plan.score);
             p.score_rows = plan.score_rows;
             p.score_pitch = plan.score_pitch;
         } else if (weight_rows > 0) {

@@ -27,9 +27,16 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnParams p) {
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, h = lane >> 5;
-    const int split = SPLIT ? blockIdx.x % p.splits : 0;
-    const int bh = SPLIT ? blockIdx.x / p.splits : blockIdx.x;
-    const int hb = bh % p.heads, b = bh / p.heads;
+    int hb = blockIdx.x % p.heads, b = blockIdx.x / p.heads, split = 0, each = 0;
+    if constexpr (SPLIT) {
+        const int parts = p.B * p.splits;
+        hb = blockIdx.x / parts;
+        const Shares shares(p, lane);
+        if (p.B > 1 && blockIdx.x == 0 && wave == 0) shares.leave(p, lane);
+        if (!shares.find(p, blockIdx.x % parts, b, split)) return;
+        each = shares.each;
+    }
+    const int bh = b * p.heads + hb;
     const SeqLens len = seq_lens(p, b);
     const int rows = p.Sq * p.pack;
 
@@ -39,7 +46,6 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnParams p) {
     const int units = (len.k + kFewKeys - 1) / kFewKeys;
     int first = 0, last = units;
     if (SPLIT) {
-        const int each = (units + p.splits - 1) / p.splits;
         first = min(units, split * each);
         last = min(units, first + each);
     }
@@ -179,7 +185,7 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnParams p) {
             for (int i = 0; i < 4; ++i) x[i] += a * y[i];
         }
         if constexpr (SPLIT) {
-            const int64_t at = ((int64_t)bh * p.splits + split) * rows + r;
+            const int64_t at = (int64_t)blockIdx.x * rows + r;
             *reinterpret_cast<f32x4*>(p.part_o + at * D + c) = x;
             if (c == 0) *reinterpret_cast<f32x2*>(p.part_ml + at * 2) = f32x2{m, lsum};
         } else if (c < p.D) {
@@ -230,12 +236,14 @@ __global__ __launch_bounds__(256) void attn_finish_kernel(AttnParams p, float* w
         const int b = bh / p.heads;
         // the (m, l) of the rows: 16 lanes for each
         const int row = threadIdx.x >> 4, l16 = threadIdx.x & 15;
-        const f32x2* part = reinterpret_cast<const f32x2*>(p.part_ml) + (int64_t)bh * p.splits * rows + min(row, rows - 1);
+        const int start = p.B > 1 ? p.shares[2 * b] : 0, splits = p.B > 1 ? p.shares[2 * b + 1] : p.splits;
+        const f32x2* part = reinterpret_cast<const f32x2*>(p.part_ml) +
+                            ((int64_t)(bh % p.heads) * (p.B * p.splits) + start) * rows + min(row, rows - 1);
         f32x2 parts[kMostSplits / 16];
 #pragma unroll
         for (int i = 0; i < kMostSplits / 16; ++i) {
             parts[i] = f32x2{-kInf, 0.0f};
-            if (i * 16 < p.splits && i * 16 + l16 < p.splits) parts[i] = part[(int64_t)(i * 16 + l16) * rows];
+            if (i * 16 < splits && i * 16 + l16 < splits) parts[i] = part[(int64_t)(i * 16 + l16) * rows];
         }
         const SeqLens len = seq_lens(p, b);
         if (blockIdx.x % chunks * kFinishKeys >= len.k) return;
@@ -278,14 +286,15 @@ __global__ __launch_bounds__(256) void attn_finish_kernel(AttnParams p, float* w
     const int block = blockIdx.x - p.B * p.heads * chunks;
     const int row = block % rows, bh = block / rows;
     const int hb = bh % p.heads, b = bh / p.heads;
-    const int64_t at = (int64_t)bh * p.splits * rows + row;   // of split 0
+    const int start = p.B > 1 ? p.shares[2 * b] : 0, splits = p.B > 1 ? p.shares[2 * b + 1] : p.splits;
+    const int64_t at = ((int64_t)hb * (p.B * p.splits) + start) * rows + row;   // of the first part
     const f32x2* part_ml = reinterpret_cast<const f32x2*>(p.part_ml) + at;
     const float* part_o = p.part_o + at * D + lane;
     f32x2 parts[kMostSplits / 64];
 #pragma unroll
     for (int i = 0; i < kMostSplits / 64; ++i) {
         parts[i] = f32x2{-kInf, 0.0f};
-        if (i * 64 < p.splits && i * 64 + lane < p.splits) parts[i] = part_ml[(int64_t)(i * 64 + lane) * rows];
+        if (i * 64 < splits && i * 64 + lane < splits) parts[i] = part_ml[(int64_t)(i * 64 + lane) * rows];
     }
     // kAhead of the wave's parts, and their m
     float y[kAhead][PER], ms[kAhead];
@@ -293,7 +302,7 @@ __global__ __launch_bounds__(256) void attn_finish_kernel(AttnParams p, float* w
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const int s = s0 + 4 * i;
-            if (s >= p.splits) break;
+            if (s >= splits) break;
             ms[i] = part_ml[(int64_t)s * rows][0];
 #pragma unroll
             for (int c = 0; c < PER; ++c) y[i][c] = part_o[(int64_t)s * rows * D + c * 64];
@@ -303,11 +312,11 @@ __global__ __launch_bounds__(256) void attn_finish_kernel(AttnParams p, float* w
     const f32x2 whole = whole_row<64, kMostSplits>(parts);
     const float m = whole[0], l = whole[1];
     float x[PER] = {};
-    for (int s0 = wave; s0 < p.splits; s0 += 4 * kAhead) {
+    for (int s0 = wave; s0 < splits; s0 += 4 * kAhead) {
         if (s0 > wave) read(s0);
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            if (s0 + 4 * i >= p.splits) break;
+            if (s0 + 4 * i >= splits) break;
             const float a = __builtin_amdgcn_exp2f(ms[i] - m);
 #pragma unroll
             for (int c = 0; c < PER; ++c) x[c] += a * y[i][c];

@@ -39,10 +39,12 @@ struct AttnParams {
     const uint64_t* tree;       // [B, Sq] new tokens that row i sees, or null
     // filled by the launchers
     int pack, heads, tiles, splits;
+    int unit_bits;              // splits are whole units of 1 << unit_bits keys
     int by_xcd, long_first;     // order of the blocks
     int halves;                 // blocks of 64 rows
-    float* part_o;              // [B][heads][splits][Sq * pack][DT] sums of a split
-    float* part_ml;             // [B][heads][splits][Sq * pack][2] (f m, l)
+    float* part_o;              // [heads][B * splits][Sq * pack][DT] sums of a part (attn_tile.hpp)
+    float* part_ml;             // [heads][B * splits][Sq * pack][2] (f m, l)
+    int32_t* shares;            // [B][2]: a sequence's first part and how many it has (B > 1)
     float* row_ml;              // [B][heads][Sq * pack][2] (f m, 1 / l), or null
     // f x of the first score_rows rows, -inf where masked, for the weights' sums;
     // keys of tiles that a row does not see at all may be missing
@@ -81,7 +83,7 @@ hipError_t launch_attn_finish(const AttnParams& p, float* weight, hipStream_t st
 // weight[b, head, key] += the weights of the first `rows` query rows, recomputed
 // from row_ml.
 hipError_t launch_attn_weights(const AttnParams& p, float* weight, int rows, hipStream_t st);
-constexpr int kMostSplits = 256;   // ranges of keys that an attention is split into
+constexpr int kMostSplits = 256;   // parts of one sequence
 constexpr int kScoreRows = 16;   // most rows whose scores are kept
 
 // ---- cache ----

@@ -45,11 +45,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
     const int wave_row = WK == 1 ? wave : wave & 1, wave_key = WK == 1 ? 0 : wave >> 1;   // its rows, its half of a tile's keys
 
     // Blocks go round the 8 XCDs in turn: each XCD gets a run of the heads (with
-    // their splits), so that the blocks that share keys share an L2.  Under a causal
+    // their parts), so that the blocks that share keys share an L2.  Under a causal
     // mask or documents the last tiles of all of the XCD's heads come first: they
     // see the most keys, and a long one that starts late is waited for at the end.
     // Else a head's tiles are next to each other.
-    int hs, tile;   // (sequence, head, split), and the tile of rows
+    int hs, tile;   // (sequence, head) or (head, part), and the tile of rows
     {
         const int all = p.B * p.heads * p.splits, each = all / 8;
         const int i = blockIdx.x >> 3, x = blockIdx.x & 7;
@@ -62,9 +62,15 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
         }
         tile = p.tiles - 1 - tile;
     }
-    const int split = SPLIT ? hs % p.splits : 0;
-    if (SPLIT) hs /= p.splits;
-    const int hb = hs % p.heads, b = hs / p.heads;
+    int hb = hs % p.heads, b = hs / p.heads, split = 0, each = 0;
+    if constexpr (SPLIT) {   // hs: (head, part)
+        const int parts = p.B * p.splits;
+        hb = hs / parts;
+        const Shares shares(p, lane);
+        if (p.B > 1 && blockIdx.x == 0 && wave == 0) shares.leave(p, lane);
+        if (!shares.find(p, hs % parts, b, split)) return;
+        each = shares.each;
+    }
     const SeqLens len = seq_lens(p, b);
     const int rows = len.q * p.pack;
     const int row0 = tile * (kSeqTileRows / WK);
@@ -97,7 +103,6 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
     const int kend = p.causal ? min(len.k, max(bpos1 + 1, prefix)) : len.k;
     int first = 0, last = (kend + kTileKeys - 1) / kTileKeys;   // tiles
     if (SPLIT) {
-        const int each = (last + p.splits - 1) / p.splits;
         first = min(last, split * each);
         last = min(last, first + each);
     }
@@ -413,7 +418,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
     if (!has_row) return;
     const late_params_t e = late_params();
     if constexpr (SPLIT) {
-        const int64_t at = ((int64_t)(b * e->heads + hb) * e->splits + split) * ((int64_t)e->Sq * e->pack) + row;
+        const int64_t at = (int64_t)hs * ((int64_t)e->Sq * e->pack) + row;
         float* po = e->part_o + at * D;
 #pragma unroll
         for (int db = 0; db < DB; ++db)

@@ -185,6 +185,35 @@ def test_chunk_in_two_calls(pkg, dev, T, n):
     assert torch.equal(cache.weight[0, 0, :, 37 + T:], before[0, 0, :, 37 + T:])
 
 
+@pytest.mark.parametrize("B,Hk,T,rows", [(2, 4, 1, 1), (5, 1, 1, 0), (70, 1, 1, 1), (130, 1, 3, 3), (3, 2, 23, 1),
+                                         (70, 1, 23, 23), (4, 1, 40, 0)])
+def test_unequal_lengths(pkg, dev, B, Hk, T, rows):
+    """Parts are shared out by length: sequences from nothing to thousands of tokens in
+    one call, every one against the plain attention."""
+    import torch
+    gen = torch.Generator().manual_seed(B)
+    capacity = 6000 if B < 10 else 900
+    lens = torch.randint(0, capacity // 8, (B,), generator=gen)
+    lens[0], lens[-1] = 0, capacity - T       # one empty, one that fills the cache
+    cache = _cache(pkg, dev, 1, lens.tolist(), Hk, capacity, 64, weights=True)
+    before = cache.weight.clone()
+    q = torch.randn(B, T, 4 * Hk, 64, device=dev).half()
+    out = pkg.attention_cached(q, cache, 0, 0.25, weight_rows=rows)
+    for b in range(B):
+        n = int(lens[b])
+        j, t = torch.arange(n + T, device=dev)[None] - n, torch.arange(T, device=dev)[:, None]
+        for g in range(Hk):
+            want = torch.zeros(n + T, dtype=torch.float64, device=dev)
+            for h in range(4 * g, 4 * g + 4):
+                p, ref, _, bound = R.head(q[b, :, h], cache.k[0, b, g, :n + T], cache.v[0, b, g, :n + T], 0.25, 0.0,
+                                          None, j <= t)
+                R.check_out(out[b, :, h], ref, bound, q.dtype, (b, h))
+                want += p[:rows].sum(0)
+            d = (cache.weight[0, b, g, :n + T].double() - before[0, b, g, :n + T].double() - want).abs()
+            assert (d <= 2.0 ** -22 * (1 + want) + 1e-5 * want).all(), (b, g)
+            assert torch.equal(cache.weight[0, b, g, n + T:], before[0, b, g, n + T:])
+
+
 def test_full_cache(pkg, dev):
     """Tokens past the capacity are dropped: not written, not seen, not counted."""
     import torch
