@@ -200,7 +200,8 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnParams p) {
 
 // The end of a split attention.  A block for each row: out = sum over the splits of
 // exp2(m_s - m) part_s, divided by the same sum of their l; four waves take every
-// fourth split.  Blocks ahead of them take 1024 keys of a head each, and add the
+// fourth split.  Or a wave for each row, ROWS = 4 to a block, where those are
+// enough.  Blocks ahead of them take 1024 keys of a head each, and add the
 // weights of the rows whose scores were kept, exp2(f x - m) / l summed over the
 // rows.  What a block reads does not depend on what it computes, so all of it is on
 // its way at once: the launch is one trip to memory long.
@@ -223,10 +224,10 @@ __device__ __forceinline__ f32x2 whole_row(const f32x2 (&x)[MOST / EVERY]) {
     return f32x2{m, l};
 }
 
-template <int D, bool BF>
+template <int D, bool BF, int ROWS>
 __global__ __launch_bounds__(256) void attn_finish_kernel(AttnParams p, float* weight) {
     constexpr int PER = D / 64;
-    __shared__ float sums[4][D];
+    __shared__ __attribute__((aligned(8))) float sums[ROWS == 1 ? 4 : 1][D];
     __shared__ f32x2 ml[kScoreRows];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rows = p.Sq * p.pack;
@@ -283,13 +284,18 @@ __global__ __launch_bounds__(256) void attn_finish_kernel(AttnParams p, float* w
             if (j + e < len.k) w[e] = old[e] + sum[e];
         return;
     }
-    const int block = blockIdx.x - p.B * p.heads * chunks;
-    const int row = block % rows, bh = block / rows;
+    // the wave's row, and its parts: every fourth one, or all
+    const int block = blockIdx.x - p.B * p.heads * chunks, index = ROWS == 1 ? block : block * ROWS + wave;
+    constexpr int STEP = 4 / ROWS;
+    const int first = ROWS == 1 ? wave : 0;
+    if (index >= p.B * p.heads * rows) return;
+    const int row = index % rows, bh = index / rows;
     const int hb = bh % p.heads, b = bh / p.heads;
     const int start = p.B > 1 ? p.shares[2 * b] : 0, splits = p.B > 1 ? p.shares[2 * b + 1] : p.splits;
     const int64_t at = ((int64_t)hb * (p.B * p.splits) + start) * rows + row;   // of the first part
     const f32x2* part_ml = reinterpret_cast<const f32x2*>(p.part_ml) + at;
-    const float* part_o = p.part_o + at * D + lane;
+    typedef float vec __attribute__((ext_vector_type(PER)));   // columns PER lane ..
+    const vec* part_o = reinterpret_cast<const vec*>(p.part_o + at * D) + lane;
     f32x2 parts[kMostSplits / 64];
 #pragma unroll
     for (int i = 0; i < kMostSplits / 64; ++i) {
@@ -297,44 +303,45 @@ __global__ __launch_bounds__(256) void attn_finish_kernel(AttnParams p, float* w
         if (i * 64 < splits && i * 64 + lane < splits) parts[i] = part_ml[(int64_t)(i * 64 + lane) * rows];
     }
     // kAhead of the wave's parts, and their m
-    float y[kAhead][PER], ms[kAhead];
+    vec y[kAhead];
+    float ms[kAhead];
     auto read = [&](int s0) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const int s = s0 + 4 * i;
+            const int s = s0 + STEP * i;
             if (s >= splits) break;
             ms[i] = part_ml[(int64_t)s * rows][0];
-#pragma unroll
-            for (int c = 0; c < PER; ++c) y[i][c] = part_o[(int64_t)s * rows * D + c * 64];
+            y[i] = part_o[(int64_t)s * rows * 64];
         }
     };
-    read(wave);
+    read(first);
     const f32x2 whole = whole_row<64, kMostSplits>(parts);
     const float m = whole[0], l = whole[1];
-    float x[PER] = {};
-    for (int s0 = wave; s0 < splits; s0 += 4 * kAhead) {
-        if (s0 > wave) read(s0);
+    vec x = {};
+    for (int s0 = first; s0 < splits; s0 += STEP * kAhead) {
+        if (s0 > first) read(s0);
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            if (s0 + 4 * i >= splits) break;
-            const float a = __builtin_amdgcn_exp2f(ms[i] - m);
-#pragma unroll
-            for (int c = 0; c < PER; ++c) x[c] += a * y[i][c];
+            if (s0 + STEP * i >= splits) break;
+            x += __builtin_amdgcn_exp2f(ms[i] - m) * y[i];
         }
     }
+    if constexpr (ROWS == 1) {
+        reinterpret_cast<vec*>(sums[wave])[lane] = x;
+        __syncthreads();
+        if (wave > 0) return;
+        x = vec{};
 #pragma unroll
-    for (int i = 0; i < PER; ++i) sums[wave][i * 64 + lane] = x[i];
-    __syncthreads();
+        for (int w = 0; w < 4; ++w) x += reinterpret_cast<const vec*>(sums[w])[lane];
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (p.row_ml && threadIdx.x == 0)
-        *reinterpret_cast<f32x2*>(p.row_ml + ((int64_t)bh * rows + row) * 2) = f32x2{l == 0.0f ? 0.0f : m, inv};
-    const int c = threadIdx.x * 2;
-    if (c < p.D) {
-        const float y0 = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
-        const float y1 = (sums[0][c + 1] + sums[1][c + 1]) + (sums[2][c + 1] + sums[3][c + 1]);
+    if (p.row_ml && lane == 0)
+        *reinterpret_cast<f32x2*>(p.row_ml + (int64_t)index * 2) = f32x2{l == 0.0f ? 0.0f : m, inv};
+    if (lane * PER < p.D) {
         uint16_t* out = p.out + b * p.os.b + (int64_t)(row / p.pack) * p.os.r +
-                        (int64_t)(hb * p.pack + row % p.pack) * p.os.h;
-        *reinterpret_cast<uint32_t*>(out + c) = pack2<BF>(y0 * inv, y1 * inv);
+                        (int64_t)(hb * p.pack + row % p.pack) * p.os.h + lane * PER;
+        if constexpr (PER == 2) *reinterpret_cast<uint32_t*>(out) = pack2<BF>(x[0] * inv, x[1] * inv);
+        else *out = (uint16_t)pack2<BF>(x[0] * inv, 0.0f);
     }
 }
 
@@ -411,19 +418,25 @@ hipError_t launch_attn_few(AttnParams p, hipStream_t st) {
     return p.bf16 ? launch_few<64, true>(p, st) : launch_few<64, false>(p, st);
 }
 
-hipError_t launch_attn_finish(const AttnParams& p, float* weight, hipStream_t st) {
+template <int D, bool BF>
+static hipError_t launch_finish(const AttnParams& p, float* weight, hipStream_t st) {
     const int chunks = p.scores ? (p.Sk + kFinishKeys - 1) / kFinishKeys : 0;
-    const int64_t blocks = (int64_t)p.B * p.heads * (p.Sq * p.pack + chunks);
+    const int64_t heads = (int64_t)p.B * p.heads, rows = heads * p.Sq * p.pack;
+    // A wave for each row from four blocks of them for each CU on.  Measured (one wave /
+    // four, us of the whole call): 40 rows for 4 sequences of 12000 keys and 24 heads of
+    // 128 50.0 / 52.4; 16 rows for 8 sequences of 3000 28.5 / 30.7; fewer rows leave CUs idle.
+    const bool many = rows >= 4 * kCUs;
+    const int64_t blocks = heads * chunks + (many ? (rows + 3) / 4 : rows);
     if (blocks > 0x7fffff00 / 256) return hipErrorInvalidValue;
     const dim3 g((unsigned)blocks), t(256);
-    if (p.D > 64) {
-        if (p.bf16) hipLaunchKernelGGL((attn_finish_kernel<128, true>), g, t, 0, st, p, weight);
-        else hipLaunchKernelGGL((attn_finish_kernel<128, false>), g, t, 0, st, p, weight);
-    } else {
-        if (p.bf16) hipLaunchKernelGGL((attn_finish_kernel<64, true>), g, t, 0, st, p, weight);
-        else hipLaunchKernelGGL((attn_finish_kernel<64, false>), g, t, 0, st, p, weight);
-    }
+    if (many) hipLaunchKernelGGL((attn_finish_kernel<D, BF, 4>), g, t, 0, st, p, weight);
+    else hipLaunchKernelGGL((attn_finish_kernel<D, BF, 1>), g, t, 0, st, p, weight);
     return hipGetLastError();
+}
+
+hipError_t launch_attn_finish(const AttnParams& p, float* weight, hipStream_t st) {
+    if (p.D > 64) return p.bf16 ? launch_finish<128, true>(p, weight, st) : launch_finish<128, false>(p, weight, st);
+    return p.bf16 ? launch_finish<64, true>(p, weight, st) : launch_finish<64, false>(p, weight, st);
 }
 
 template <int D, bool BF>
