@@ -30,10 +30,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
     constexpr int TILE = kTileKeys * D;          // values of a tile
     constexpr int QT = D / 16, DB = D / 32, KB = 2 / WK;   // KB blocks of 32 keys a wave and tile
     constexpr int INSTR = TILE * 2 / 1024 / 4;   // copies of a wave into a tile
-    // Stages: with three the copies are two tiles ahead, which a block that runs
-    // alone on its CU needs (a tile of 1.05 us waits for memory most of it); at
-    // head_dim 128 a third would leave room for one block on a CU instead of two.
-    constexpr int STAGES = D == 64 ? 3 : 2;
+    // Two stages.  A third changed nothing (6144 rows of 32 heads of 64: 350 us with
+    // three, 347 with two; 4095 rows of documents 62 and 61): other blocks of the CU
+    // compute while one waits.
+    constexpr int STAGES = 2;
     __shared__ __attribute__((aligned(1024))) uint16_t ks[STAGES][TILE], vs[STAGES][TILE];
     __shared__ DocTiles docs;
     __shared__ __attribute__((aligned(8))) float half_ml[WK == 2 ? 2 : 1][32][2];   // (m, l) of the second half's rows
@@ -239,27 +239,22 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
     if (cur.t < last) {
         copy(cur.t, 0);
         nxt = advance();
-        if (STAGES == 3 && nxt.t < last) copy(nxt.t, 1);
     }
-    for (int stage = 0; cur.t < last; stage = stage + 1 == STAGES ? 0 : stage + 1) {
+    for (int stage = 0; cur.t < last; stage ^= 1) {
         const int j0 = cur.t * kTileKeys, j1 = j0 + kTileKeys - 1;
         // does every row of the block see every key of the tile?
         const bool some = !(j1 < len.k && (!p.causal || j1 <= bpos0 || j1 < prefix) &&
                             cur.one_b && (!(SPLIT && p.tree) || j1 < len.old));
         partly |= some;
         if (careful && threadIdx.x < 2) bad_keys[stage][threadIdx.x] = 0;
-        // This tile is in LDS, and the stage of the one before is free.  (A wave of
-        // the first may have a copy of documents more in flight: it waits longer.)
-        // The tile before's scores, 8 stores (4 with WK = 2) and the last that the wave issued, need not
-        // have arrived.
-        if (STAGES == 3 && nxt.t < last) copies_wait<2 * INSTR>();
-        else if (STAGES == 2 && SPLIT && stored) copies_wait<4 * KB>();
+        // This tile is in LDS, and the stage of the one before is free.  The tile
+        // before's scores, 8 stores (4 with WK = 2) and the last that the wave issued,
+        // need not have arrived.
+        if (SPLIT && stored) copies_wait<4 * KB>();
         else copies_wait<0>();
         if constexpr (SPLIT) stored = false;
         __syncthreads();
-        Tile far = nxt;
-        if (STAGES == 3 && nxt.t < last) far = advance();
-        if (far.t < last) copy(far.t, stage == 0 ? STAGES - 1 : stage - 1);
+        if (nxt.t < last) copy(nxt.t, stage ^ 1);
         if (careful && some) {
 #pragma unroll
             for (int i = 0; i < TILE / 8 / 256; ++i) {
@@ -361,7 +356,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
             }
         }
         cur = nxt;
-        nxt = STAGES == 3 || !(nxt.t < last) ? far : advance();
+        if (nxt.t < last) nxt = advance();
     }
     if (careful || !partly) break;
     float any = 0.0f * st.l;   // NaN where a sum is infinite or NaN
