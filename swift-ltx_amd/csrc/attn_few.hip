@@ -349,53 +349,71 @@ __global__ __launch_bounds__(256) void attn_finish_kernel(AttnParams p, float* w
 // and read 8 bytes for each; reading K again is 2 head_dim for all of them):
 // weight[key] += sum over rows r < wrows of exp2(f x_r - mf_r) / l_r.  S = Q K^T
 // this way round, so that a lane holds 16 rows of one key: the sum over rows is
-// its own.  A wave takes 32 keys; K's fragments come straight from memory.
+// its own.  A wave takes kWeightTiles times 32 keys, for which it reads 32 rows of
+// Q and their statistics once; all fragments come straight from memory.
+constexpr int kWeightTiles = 2;
 template <int D, bool BF, bool CAP>
 __global__ __launch_bounds__(256) void attn_weights_kernel(AttnParams p, float* weight, int wrows) {
-    constexpr int QT = D / 16;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int QT = D / 16, KEYS = 32 * kWeightTiles;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, h = lane >> 5;
     const int bh = blockIdx.y, hb = bh % p.heads, b = bh / p.heads;
     const SeqLens len = seq_lens(p, b);
     const int rows = p.Sq * p.pack;
     const float f = CAP ? kLog2e : p.scale * kLog2e;
     const float yscale = CAP ? p.scale / p.cap : 0.0f;
-    const float* row_ml = p.row_ml + (int64_t)bh * rows * 2;
-    for (int j0 = (blockIdx.x * 4 + wave) * 32; j0 < len.k; j0 += gridDim.x * 128) {
-        const int j = j0 + n, jc = min(j, len.k - 1);
-        const uint16_t* k = p.k + b * p.ks.b + hb * p.ks.h + jc * p.ks.r;
-        u32x4 kf[QT];
+    const f32x2* row_ml = reinterpret_cast<const f32x2*>(p.row_ml) + (int64_t)bh * rows;
+    for (int j0 = (blockIdx.x * 4 + wave) * KEYS; j0 < len.k; j0 += gridDim.x * 4 * KEYS) {
+        const bool all = j0 + KEYS <= len.old;   // every row sees every key
+        u32x4 kf[kWeightTiles][QT];
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
-            const int c = 16 * t + 8 * h;
-            kf[t] = c < p.D ? *reinterpret_cast<const u32x4*>(k + c) : u32x4{};
+        for (int kt = 0; kt < kWeightTiles; ++kt) {
+            const uint16_t* k = p.k + b * p.ks.b + hb * p.ks.h + min(j0 + 32 * kt + n, len.k - 1) * p.ks.r;
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                const int c = 16 * t + 8 * h;
+                kf[kt][t] = c < p.D ? *reinterpret_cast<const u32x4*>(k + c) : u32x4{};
+            }
         }
-        float sum = 0.0f;
+        float sum[kWeightTiles] = {};
         for (int r0 = 0; r0 < wrows; r0 += 32) {
             const int r = min(r0 + n, wrows - 1);
             const uint16_t* q = p.q + b * p.qs.b + (int64_t)(r / p.pack) * p.qs.r +
                                 (int64_t)(hb * p.pack + r % p.pack) * p.qs.h;
-            f32x16 s = {};
+            u32x4 qf[QT];
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
                 const int c = 16 * t + 8 * h;
-                const u32x4 qf = c < p.D ? *reinterpret_cast<const u32x4*>(q + c) : u32x4{};
-                s = mfma32<BF>(qf, kf[t], s);
+                qf[t] = c < p.D ? *reinterpret_cast<const u32x4*>(q + c) : u32x4{};
             }
+            f32x2 ml[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int row = r0 + 8 * (i / 4) + 4 * h + i % 4;
-                if (row < wrows) {
-                    const int t = row / p.pack;
-                    const bool sees = j < len.k && cached_sees(p, len, b, t, j);
+                ml[i] = row_ml[min(row, wrows - 1)];
+                if (row >= wrows) ml[i][1] = 0.0f;
+            }
+#pragma unroll
+            for (int kt = 0; kt < kWeightTiles; ++kt) {
+                f32x16 s = {};
+#pragma unroll
+                for (int t = 0; t < QT; ++t) s = mfma32<BF>(qf[t], kf[kt][t], s);
+                const int j = j0 + 32 * kt + n;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
                     const float x = CAP ? capped(s[i] * yscale, p.cap) : s[i];
-                    const f32x2 ml = *reinterpret_cast<const f32x2*>(row_ml + row * 2);
-                    sum += sees ? __builtin_amdgcn_exp2f(x * f - ml[0]) * ml[1] : 0.0f;
+                    const int row = min(r0 + 8 * (i / 4) + 4 * h + i % 4, wrows - 1);
+                    const bool sees = (all || (j < len.k && cached_sees(p, len, b, row / p.pack, j))) && ml[i][1] != 0.0f;
+                    sum[kt] += sees ? __builtin_amdgcn_exp2f(x * f - ml[i][0]) * ml[i][1] : 0.0f;
                 }
             }
         }
-        sum = half_sum(sum);
-        if (j < len.k && h == 0) weight[(int64_t)bh * p.Sk + j] += sum;
+#pragma unroll
+        for (int kt = 0; kt < kWeightTiles; ++kt) {
+            const int j = j0 + 32 * kt + n;
+            const float w = half_sum(sum[kt]);
+            if (j < len.k && h == 0) weight[(int64_t)bh * p.Sk + j] += w;
+        }
     }
 }
 
@@ -441,7 +459,7 @@ hipError_t launch_attn_finish(const AttnParams& p, float* weight, hipStream_t st
 
 template <int D, bool BF>
 static hipError_t launch_weights(const AttnParams& p, float* weight, int wrows, hipStream_t st) {
-    const dim3 g(std::min(64, (p.Sk + 127) / 128), p.B * p.heads), t(256);
+    const dim3 g(std::min(64, (p.Sk + 128 * kWeightTiles - 1) / (128 * kWeightTiles)), p.B * p.heads), t(256);
     if (p.cap > 0.0f) hipLaunchKernelGGL((attn_weights_kernel<D, BF, true>), g, t, 0, st, p, weight, wrows);
     else hipLaunchKernelGGL((attn_weights_kernel<D, BF, false>), g, t, 0, st, p, weight, wrows);
     return hipGetLastError();
