@@ -362,7 +362,9 @@ __device__ __forceinline__ int wave_scan(int x) {
 // for.  `each` is as small as the parts allow: with ceil(all / parts) one sequence
 // or another may need a part more than there is, with ceil(all / (parts - B)) none
 // does.  A lane holds the parts of `per` sequences (one, up to 64 sequences).
-// Measured: 4 sequences of 8150 to 16301 tokens, XX us instead of XX with as many parts each.
+// Measured against as many parts for each (24 heads of 128): one sequence of 16000 and
+// seven of 1000 tokens 27.7 us instead of 33.0 for a token each, 31.1 instead of 67.1
+// for 16; eight of 3000 the same.
 struct Shares {
     int each, per;
     int before, mine;   // parts of the sequences before the lane's, and of its own
