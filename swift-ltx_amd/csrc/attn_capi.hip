@@ -2,7 +2,9 @@
 // validation, the choice of kernel, launches.  Validation runs before any HIP
 // call.
 #include <algorithm>
+#include <array>
 #include <cmath>
+#include <utility>
 
 #include "attn_launch.hpp"
 #include "q4_common.hpp"
@@ -52,6 +54,21 @@ bool overlap(const Tensor& a, const Tensor& b) {
     return x < y + b.span() && y < x + a.span();
 }
 
+// Whether rows of a tensor share memory: its dimensions, from the smallest stride on,
+// have to step over all of those before.
+bool rows_share(const Tensor& t) {
+    std::array<std::pair<int64_t, int64_t>, 3> dims = {
+        {{t.stride[0], t.batch}, {t.stride[1], t.rows}, {t.stride[2], t.heads}}};
+    std::sort(dims.begin(), dims.end());
+    int64_t span = t.dim;
+    for (const auto& [stride, n] : dims) {
+        if (n <= 1) continue;
+        if (stride < span) return true;
+        span += stride * (n - 1);
+    }
+    return false;
+}
+
 int check_heads(const char* fn, int dtype, int q_heads, int kv_heads, int head_dim) {
     if (dtype != SLTX_F16 && dtype != SLTX_BF16)
         return set_error(kErrInvalid, "%s: dtype %d must be SLTX_F16 or SLTX_BF16", fn, dtype);
@@ -67,6 +84,10 @@ int check_scores(const char* fn, float scale, float softcap) {
         return set_error(kErrInvalid, "%s: scale must be positive and finite", fn);
     if (!(softcap >= 0.0f) || !std::isfinite(softcap))
         return set_error(kErrInvalid, "%s: softcap must be finite and not negative (0: none)", fn);
+    // what the kernels form of them: 2 log2(e) scale / softcap, 2 log2(e) softcap
+    if (!std::isfinite(3.0f * scale) || !std::isfinite(3.0f * softcap) ||
+        (softcap > 0.0f && !std::isfinite(3.0f * scale / softcap)))
+        return set_error(kErrUnsupported, "%s: scale %g with softcap %g leaves fp32's range", fn, scale, softcap);
     return kOk;
 }
 
@@ -180,12 +201,11 @@ int sltx_attention(const sltx_attention_args* a, void* stream) {
         return rc;
     if (overlap(out, q) || (a->k_rows > 0 && (overlap(out, k) || overlap(out, v))))
         return set_error(kErrInvalid, "%s: out overlaps q, k or v", fn);
-    // rows of out must not share memory
-    if ((a->q_heads > 1 && a->out_stride[2] < a->head_dim) || (a->q_rows > 1 && a->out_stride[1] < a->head_dim) ||
-        (a->batch > 1 && a->out_stride[0] < a->head_dim))
-        return set_error(kErrInvalid, "%s: out's rows overlap each other", fn);
+    if (rows_share(out)) return set_error(kErrInvalid, "%s: out's rows overlap each other", fn);
     if (a->bias && (a->bias_len <= 0 || a->bias_zero < 0 || a->bias_zero >= a->bias_len || a->bias_head_stride < 0))
         return set_error(kErrInvalid, "%s: bias of %d values with distance 0 at %d", fn, a->bias_len, a->bias_zero);
+    if (a->bias && a->bias_len > (1 << 30))
+        return set_error(kErrUnsupported, "%s: a bias of %d distances", fn, a->bias_len);
     if (a->prefix && !a->causal) return set_error(kErrInvalid, "%s: a prefix needs causal", fn);
     if ((a->q_docs == nullptr) != (a->k_docs == nullptr))
         return set_error(kErrInvalid, "%s: q_docs and k_docs go together", fn);

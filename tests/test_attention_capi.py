@@ -54,6 +54,12 @@ def _args(pkg, **kw):
     (dict(out=A + 0x100000), -1, "overlaps"),
     (dict(out_stride=(1024, 256, 0)), -1, "overlap each other"),
     (dict(out_stride=(1024, 0, 64)), -1, "overlap each other"),
+    (dict(out_stride=(1024, 64, 64)), -1, "overlap each other"),
+    (dict(out_stride=(64, 256, 64), batch=2), -1, "overlap each other"),
+    (dict(softcap=1e-38, scale=8.0), -2, "fp32's range"),
+    (dict(softcap=2e38), -2, "fp32's range"),
+    (dict(scale=3e38), -2, "fp32's range"),
+    (dict(bias=FAR, bias_len=(1 << 30) + 1, bias_zero=0), -2, "distances"),
     (dict(bias=A, bias_len=0), -1, "bias"),
     (dict(bias=A, bias_len=5, bias_zero=5), -1, "bias"),
     (dict(bias=A, bias_len=5, bias_zero=-1), -1, "bias"),
@@ -151,6 +157,7 @@ def test_no_cache_and_empty_cache(pkg, call):
     (dict(heads=5), -1, "not a multiple"),
     (dict(scale=0.0), -1, "scale"),
     (dict(cap=-1.0), -1, "softcap"),
+    (dict(cap=1e-38, scale=8.0), -2, "fp32's range"),
     (dict(tokens=65, tree=A), -1, "tree"),
     (dict(tree=A + 4), -1, "tree"),
     (dict(rows=5), -1, "weights"),
