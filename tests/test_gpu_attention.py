@@ -237,6 +237,21 @@ def test_strides(pkg, dev):
     _check(pkg, dev, q, one, v, 0.2)
 
 
+def test_far_offsets(pkg, dev):
+    """Keys, values and rows 2^20 values apart: offsets past 2^32 bytes and 2^31 values."""
+    import torch
+    rows, gap, D = 2100, 1 << 20, 64
+    base = torch.empty(rows * gap, dtype=torch.float16, device=dev)
+    assert base.numel() > 2 ** 31
+    q, k, v, out = (base.as_strided((1, rows, 2, D), (rows * gap, gap, D, 1), 256 * i) for i in range(4))
+    gen = torch.Generator(device=dev).manual_seed(5)
+    for x in (q, k, v):
+        x.copy_(torch.randn(1, rows, 2, D, generator=gen, device=dev))
+    with pytest.raises(pkg.SltxError):
+        pkg.attention(q, k, v, 0.2, causal=True, out=out)     # its span holds q's
+    _check(pkg, dev, q, k, v, 0.2, causal=True)
+
+
 def test_large_and_equal_scores(pkg, dev):
     """A growing maximum (late keys dominate), and scores that are all equal."""
     import torch

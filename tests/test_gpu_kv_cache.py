@@ -325,6 +325,50 @@ def test_accept_counts(pkg, dev):
     assert cache.length.tolist() == [15, 15, 16, 16]
 
 
+def test_far_offsets(pkg, dev):
+    """A cache of more than 2^31 values: its last layer and head, near the end of
+    hundreds of thousands of slots, through all the operators."""
+    import torch
+    L, Hk, C, D, n, T = 4, 8, 600_064, 128, 600_000, 3
+    k, v = (torch.empty(L, 1, Hk, C, D, dtype=torch.float16, device=dev) for _ in range(2))
+    assert k.numel() > 2 ** 31
+    gen = torch.Generator(device=dev).manual_seed(3)
+    lay = L - 1
+    for x in (k, v):
+        x[lay].normal_(generator=gen)
+    weight = torch.zeros(L, 1, Hk, C, device=dev)
+    weight[lay] = torch.rand(1, Hk, C, generator=gen, device=dev)
+    position = torch.arange(C, dtype=torch.int32, device=dev).repeat(L, 1, Hk, 1)
+    counts = torch.tensor([[n], [n]], dtype=torch.int32, device=dev)
+    cache = pkg.KVCache.from_tensors(k, v, counts, weight=weight, position=position)
+    new = torch.randn(1, T, 3 * Hk, D, generator=gen, device=dev).half()
+    q = pkg.kv_append(new[:, :, :Hk], new[:, :, Hk:2 * Hk], new[:, :, 2 * Hk:], cache, lay)
+    assert torch.equal(k[lay, 0, :, n:n + T], new[0, :, Hk:2 * Hk].transpose(0, 1))
+    assert torch.equal(v[lay, 0, :, n:n + T], new[0, :, 2 * Hk:].transpose(0, 1))
+    out = pkg.attention_cached(q, cache, lay, 0.3)
+    seen = torch.arange(n + T, device=dev)[None] <= n + torch.arange(T, device=dev)[:, None]
+    for h in (0, Hk - 1):
+        _, ref, _, bound = R.head(q[0, :, h], k[lay, 0, h, :n + T], v[lay, 0, h, :n + T], 0.3, 0.0, None, seen)
+        R.check_out(out[0, :, h], ref, bound, q.dtype, h)
+    want = k[lay, 0, :, n + 2].clone()
+    pkg.kv_accept(cache, T, path=torch.tensor([[0, 2]], dtype=torch.int32, device=dev))
+    assert cache.length.tolist() == [n + 2] and torch.equal(k[lay, 0, :, n + 1], want)
+    budget, w = 500_000, weight[lay, 0, Hk - 1, :n + 2].clone()
+    last = n + 2 - 8                       # protected: the first 4 and the last 8 positions
+    w[:4] = w[last:] = 2.0
+    keep = torch.zeros(n + 2, dtype=torch.bool, device=dev)
+    keep[torch.sort(w, descending=True, stable=True).indices[:budget]] = True
+    holes = torch.nonzero(~keep[:budget])[:, 0]
+    comers = budget + torch.nonzero(keep[budget:])[:, 0]
+    slots = torch.arange(budget, device=dev)
+    slots[holes] = comers
+    want, at = k[lay, 0, Hk - 1].index_select(0, slots), position[lay, 0, Hk - 1][slots]
+    pkg.kv_evict(cache, budget, sinks=4, recent=8)
+    assert cache.length.tolist() == [budget]
+    assert torch.equal(position[lay, 0, Hk - 1, :budget], at)
+    assert torch.equal(k[lay, 0, Hk - 1, :budget], want)
+
+
 # ---- evict ----
 
 def _evicted(w, p, n, after, budget, sinks, recent, C):
