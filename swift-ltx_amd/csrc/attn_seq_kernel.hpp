@@ -180,12 +180,23 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
     auto look = [&](int at) __attribute__((always_inline)) {   // all threads: fills docs for tiles at .. at + 63
         const int t = threadIdx.x >> 2, j = (at + t) * kTileKeys + (threadIdx.x & 3) * 16;
         int lo = 0x7fffffff, hi = -1, low = 0x7fffffff;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const int k = kdocs[min(j + e, kend - 1)], d = j + e < kend ? k : -1;
+        auto take = [&](int d) __attribute__((always_inline)) {
             lo = min(lo, d < 0 ? 0x7fffffff : d);
             low = min(low, d);
             hi = max(hi, d);
+        };
+        // four ids a load (4-byte aligned); the last ones are read again rather than past the end
+        typedef int ids __attribute__((ext_vector_type(4), aligned(4)));
+        if (kend >= 4) {
+            ids d[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) d[g] = *reinterpret_cast<const ids*>(kdocs + min(j + 4 * g, kend - 4));
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) take(min(j + 4 * g, kend - 4) + e >= j + 4 * g ? d[g][e] : -1);
+        } else {
+            for (int e = 0; e < 16; ++e) take(j + e < kend ? kdocs[j + e] : -1);
         }
 #pragma unroll
         for (int o = 1; o < 4; o <<= 1) {
