@@ -69,6 +69,17 @@ __device__ __forceinline__ SeqLens seq_lens(const AttnParams& p, int b) {
     return s;
 }
 
+// Sums over the lanes up to this one.
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // from 1, 2, 4, 8 lanes below in a row of 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // from the last lane of the row below
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // from lane 31
+    return x;
+}
+
 constexpr int kSeqTileRows = 128;   // query rows of a block of attn_seq_kernel.hpp
 constexpr int kTileKeys = 64;       // keys of its tiles
 constexpr int kFewRows = 32;        // most rows of a block of attn_few.hip

@@ -346,17 +346,6 @@ __device__ __forceinline__ bool cached_sees(const AttnParams& p, const SeqLens& 
     return p.tree ? (p.tree[b * (int64_t)p.Sq + t] >> (u & 63) & 1) != 0 : u <= t;
 }
 
-// Sums over the lanes up to this one.
-__device__ __forceinline__ int wave_scan(int x) {
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);   // from 1, 2, 4, 8 lanes below in a row of 16
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // from the last lane of the row below
-    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // from lane 31
-    return x;
-}
-
 // How the B * splits parts of a head are shared out: every part takes `each` units of
 // one sequence's keys, so that long sequences have more of them and none is waited
 // for.  `each` is as small as the parts allow: with ceil(all / parts) one sequence

@@ -291,7 +291,7 @@ hipError_t launch_kv_accept(const CacheParams& c, int drafted, const int32_t* pa
 // four digits of 8 bits, then one pass in slot order for the holes (slots below
 // the budget whose entry goes) and the comers (entries from slots above it that
 // stay), which a second launch moves into them.  A chain of short steps: 1792 times
-// 1025 entries 10.9 us, 128 times 6001 10.9; to start the digits at the first bit in
+// 1025 entries 10.0 us, 128 times 6001 9.4; to start the digits at the first bit in
 // which the keys differ (fewer of them, fewer equal ones) gave nothing.
 struct EvictParams {
     CacheParams c;
@@ -309,12 +309,13 @@ __device__ __forceinline__ uint32_t evict_key(const EvictParams& p, int32_t at, 
 // A block for each layer, sequence and head.  Wave w takes the slots from w * 64 R
 // on, R at a time in each lane; their keys are read once and kept in registers
 // where R covers them (up to 16384 entries: R = 16 with 16 waves), else (R = 0)
-// read again in each of the seven passes.  Measured, the whole call: 128 times 6001
-// entries 29.2 us with R = 8, 33.9 with R = 0; 1792 times 1025 entries 22.1 with 4
-// waves and R = 8, 44.2 with 16 waves, 33.9 with those and R = 0.
+// read again in each of the seven passes.  Measured, the whole call with steps of a
+// digit 0.2 us longer than now: 128 times 6001 entries 29.2 us with R = 8, 33.9 with
+// R = 0; 1792 times 1025 entries 22.1 with 4 waves and R = 8, 44.2 with 16 waves, 33.9
+// with those and R = 0.
 template <int WAVES, int R>
 __global__ __launch_bounds__(WAVES * 64) void kv_evict_select_kernel(EvictParams p) {
-    __shared__ int hist[256];
+    __shared__ int hist[2][256];   // one is cleared while the other is filled
     __shared__ int sums[WAVES][2];
     __shared__ int found[3];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -357,24 +358,20 @@ __global__ __launch_bounds__(WAVES * 64) void kv_evict_select_kernel(EvictParams
     uint32_t prefix = 0;
     int want = p.budget;   // of the keys that start with the prefix
     bool exact = false;    // every key that starts with the prefix stays
+    if (tid < 256) hist[24 >> 3 & 1][tid] = 0;
+    __syncthreads();
     for (int shift = 24; shift >= 0 && !exact; shift -= 8) {
-        for (int i = tid; i < 256; i += WAVES * 64) hist[i] = 0;
-        __syncthreads();
+        int *h = hist[shift >> 3 & 1], *other = hist[~shift >> 3 & 1];
         each([&](int, uint32_t k, bool in) {
-            if (in && (shift == 24 || k >> (shift + 8) == prefix >> (shift + 8))) atomicAdd(&hist[k >> shift & 255], 1);
+            if (in && (shift == 24 || k >> (shift + 8) == prefix >> (shift + 8))) atomicAdd(&h[k >> shift & 255], 1);
         });
+        if (tid < 256) other[tid] = 0;
         __syncthreads();
         if (wave == 0) {   // the digit in which the count from the top reaches `want`
             int c[4], sum = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum += c[i] = hist[255 - (lane * 4 + i)];
-            int before = sum;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int x = __shfl_up(before, o, 64);
-                if (lane >= o) before += x;
-            }
-            before -= sum;
+            for (int i = 0; i < 4; ++i) sum += c[i] = h[255 - (lane * 4 + i)];
+            int before = wave_scan(sum) - sum;
             if (before < want && before + sum >= want) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -392,7 +389,6 @@ __global__ __launch_bounds__(WAVES * 64) void kv_evict_select_kernel(EvictParams
         prefix |= (uint32_t)found[0] << shift;
         want = found[1];
         exact = found[2] != 0;
-        __syncthreads();
     }
     // `prefix` is the smallest key that may stay; `want` of the entries with just
     // it do, the lowest slots, or (exact) every entry from it on.
