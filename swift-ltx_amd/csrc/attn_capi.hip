@@ -268,6 +268,9 @@ int sltx_attention_cached(const void* q, const int64_t q_stride[3], const sltx_k
         (rc = check_scores(fn, scale, softcap)) != kOk)
         return rc;
     if (first < 0 || first > kMaxRows) return set_error(kErrInvalid, "%s: first token %d", fn, first);
+    if ((int64_t)tokens * (q_heads / cache->kv_heads) > kMaxRows)
+        return set_error(kErrUnsupported, "%s: %d tokens of %d query heads for each key/value head", fn, tokens,
+                         q_heads / cache->kv_heads);
     if (tree && tokens > 64) return set_error(kErrInvalid, "%s: a tree of %d tokens (64 at most)", fn, tokens);
     if (weight_rows < 0 || weight_rows > tokens)
         return set_error(kErrInvalid, "%s: weights of %d of %d tokens", fn, weight_rows, tokens);

@@ -436,11 +436,12 @@ __global__ __launch_bounds__(WAVES * 64) void kv_evict_select_kernel(EvictParams
 // the budget: 13.9 us for 57 MB read and written, 4.1 TB/s; one entry of 1792: 4.4 us.
 __global__ __launch_bounds__(256) void kv_evict_move_kernel(EvictParams p) {
     const int lbh = blockIdx.y, b = lbh / p.c.heads % p.c.B;
-    const int chunks = p.c.D / 8, moves = p.moves[lbh];
+    const uint32_t chunks = p.c.D / 8;
+    const int moves = p.moves[lbh];
     const int32_t *holes = p.holes + (int64_t)lbh * p.most, *comers = p.comers + (int64_t)lbh * p.most;
     const int64_t base = (int64_t)lbh * p.c.capacity;
-    for (int e = blockIdx.x * 256 + threadIdx.x; e < moves * chunks; e += gridDim.x * 256) {
-        const int m = e / chunks, piece = e % chunks;
+    for (uint32_t e = blockIdx.x * 256 + threadIdx.x; e < (uint32_t)moves * chunks; e += gridDim.x * 256) {
+        const uint32_t m = e / chunks, piece = e % chunks;   // up to 2^27 * 16 pieces
         const int64_t d = base + holes[m], s = base + comers[m];
         const u32x4 k = *reinterpret_cast<const u32x4*>(p.c.k + s * p.c.D + piece * 8);
         const u32x4 v = *reinterpret_cast<const u32x4*>(p.c.v + s * p.c.D + piece * 8);

@@ -154,6 +154,7 @@ def test_no_cache_and_empty_cache(pkg, call):
     (dict(layer=-1), -1, "layer"),
     (dict(tokens=-1), -1, "tokens"),
     (dict(first=-1), -1, "first"),
+    (dict(tokens=1 << 28), -2, "query heads for each"),
     (dict(heads=5), -1, "not a multiple"),
     (dict(scale=0.0), -1, "scale"),
     (dict(cap=-1.0), -1, "softcap"),
