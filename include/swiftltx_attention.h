@@ -71,6 +71,8 @@ int sltx_attention(const sltx_attention_args* args, void* stream);
  * next_position[b] is the position that the next token has, for its rotary
  * angles: larger than length[b] once entries were evicted.  The lengths live in
  * device memory, so that a captured step can be replayed as they grow.
+ * Calls over one cache share its workspace too: they run one after the other, on
+ * one stream or ordered by events.
  * weight and position (both or neither) serve eviction: of each slot the
  * attention weight that its key has had so far, and its token's position. */
 typedef struct sltx_kv_cache {

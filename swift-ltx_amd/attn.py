@@ -162,7 +162,8 @@ class KVCache:
     Every tensor stays in place for the cache's life, so steps over it can be
     captured in a HIP graph; so does every scratch buffer that a call needed (they
     grow: make a captured call once eagerly first, so that its scratch does not
-    come from the graph's own memory)."""
+    come from the graph's own memory).  Calls over one cache share its scratch: they
+    are ordered like any that write one tensor, on one stream or with events."""
 
     def __init__(self, layers, batch, kv_heads, capacity, head_dim, dtype=None, track_weights=False, device="cuda"):
         import torch
