@@ -366,6 +366,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
             }
             if (careful && some) {   // keys with infinities or NaN in their V rows
                 uint64_t bad = (uint64_t)bad_keys[stage][1] << 32 | bad_keys[stage][0];
+                // Rows that overlap (a stride below head_dim) put values of the last keys
+                // into the places of keys past the end, which have no row to read.
+                if (j1 >= len.k) bad &= (1ull << (len.k - j0)) - 1;
                 while (bad) {
                     const int j = j0 + __builtin_ctzll(bad);
                     bad &= bad - 1;
