@@ -132,7 +132,7 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnParams p) {
         for (int t = 0; t < QT; ++t) s = mfma32<BF>(k_frag<D>(kt, kfrag, 0, t), qf[t], s);
         if constexpr (CAP) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = capped(s[i] * yscale, p.cap);
+            for (int i = 0; i < 16; ++i) s[i] = capped(s[i], yscale, p.scale, p.cap);
         }
         if (!all) {
             const int d = lim - j0 - 4 * h;
@@ -413,7 +413,7 @@ __global__ __launch_bounds__(256) void attn_weights_kernel(AttnParams p, float* 
                 const int j = j0 + 32 * kt + n;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const float x = CAP ? capped(s[i] * yscale, p.cap) : s[i];
+                    const float x = CAP ? capped(s[i], yscale, p.scale, p.cap) : s[i];
                     const int row = min(r0 + 8 * (i / 4) + 4 * h + i % 4, wrows - 1);
                     const bool sees = (all || (j < len.k && cached_sees(p, len, b, row / p.pack, j))) && ml[i][1] != 0.0f;
                     sum[kt] += sees ? __builtin_amdgcn_exp2f(x * f - ml[i][0]) * ml[i][1] : 0.0f;

@@ -26,7 +26,9 @@ namespace sltx {
 
 // Variants.  Documents, and the parts that a cached attention is split into (the
 // only ones with a tree), have kernels of their own: their state costs registers.
-enum : int { kCap = 1, kBias = 2, kSplit = 4, kDocs = 8 };
+// So have caps above kShortCap (kClose, with kCap).
+enum : int { kCap = 1, kBias = 2, kSplit = 4, kDocs = 8, kClose = 16 };
+constexpr float kShortCap = 64.0f;   // models' caps are 30 and 50
 
 // Documents of a run of 64 tiles (one lane each): the smallest and largest id
 // of a tile's keys, ids below 0 (padding) left out, and whether all are equal.
@@ -37,6 +39,7 @@ struct DocTiles {
 template <int D, bool BF, int MODE, int WK>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnParams p) {
     constexpr bool CAP = MODE & kCap, BIAS = MODE & kBias, SPLIT = MODE & kSplit, DOCS = MODE & kDocs;
+    constexpr bool CLOSE = CAP && (SPLIT || MODE & kClose);
     constexpr int TILE = kTileKeys * D;          // values of a tile
     constexpr int QT = D / 16, DB = D / 32, KB = 2 / WK;   // KB blocks of 32 keys a wave and tile
     constexpr int INSTR = TILE * 2 / 1024 / 4;   // copies of a wave into a tile
@@ -244,10 +247,13 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
     RowState<BF> st;
     // Weights are exp2(f x).  A capped score is cap tanh(y) = cap - 2 cap t, with
     // t = 1 / (1 + e^(2 y)): x = -t, the constant drops out of the softmax (with a
-    // bias the score itself is formed).  Off by 9 * 2^-24 cap: enough for weights of
-    // 16 bits.  Parts may serve fp32 weights and take the closer form (capped).
-    const float f = BIAS || (CAP && SPLIT) ? kLog2e : CAP ? 2.0f * p.cap * kLog2e : p.scale * kLog2e;
-    const float capscale = !CAP ? 0.0f : SPLIT ? p.scale / p.cap : 2.0f * kLog2e * p.scale / p.cap;
+    // bias the score itself is formed).  Off by 9 * 2^-24 cap, at the largest cap that
+    // takes this form a fourteenth of what rounding to fp16 costs a weight.  Larger
+    // caps, and parts, which may serve fp32 weights, take the form that is as close at
+    // any cap (capped).  4096 causal rows of 32 heads, head_dim 64 / 128: 91 / 147 us
+    // without a cap, 120 / 183 in the short form, 160 / 219 in the other.
+    const float f = BIAS || CLOSE ? kLog2e : CAP ? 2.0f * p.cap * kLog2e : p.scale * kLog2e;
+    const float capscale = !CAP ? 0.0f : CLOSE ? p.scale / p.cap : 2.0f * kLog2e * p.scale / p.cap;
     const float* bias = BIAS ? p.bias + head * p.bias_h : nullptr;
     const uint32_t kfrag = klds + k_frag_base<D>(lane), vfrag = vlds + v_frag_base<D>(lane);
 
@@ -322,11 +328,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_seq_kernel(AttnPara
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         float x = s[kb][i];
-                        if constexpr (CAP && SPLIT) x = capped(x * capscale, p.cap);
+                        if constexpr (CLOSE) x = capped(x, capscale, p.scale, p.cap);
                         else if constexpr (CAP) x = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(x * capscale));
                         if constexpr (BIAS) {
                             const int j = jb + 8 * (i / 4) + 4 * h + i % 4;
-                            x = (CAP ? p.cap + 2.0f * p.cap * x : x * p.scale) +
+                            x = (CLOSE ? x : CAP ? p.cap + 2.0f * p.cap * x : x * p.scale) +
                                 bias[min(max(j - pos + p.bias_zero, 0), p.bias_n - 1)];
                         }
                         s[kb][i] = x;
@@ -469,7 +475,8 @@ static hipError_t launch_one(const AttnParams& p, dim3 g, hipStream_t st) {
 }
 template <int D, bool BF, int WK>
 static hipError_t launch_mode(const AttnParams& p, dim3 g, hipStream_t st) {
-    const int mode = (p.cap > 0.0f ? kCap : 0) | (p.bias ? kBias : 0) | (p.part_o ? kSplit : 0) | (p.q_docs ? kDocs : 0);
+    const int mode = (p.cap > 0.0f ? kCap : 0) | (p.cap > kShortCap && !p.part_o ? kClose : 0) | (p.bias ? kBias : 0) |
+                     (p.part_o ? kSplit : 0) | (p.q_docs ? kDocs : 0);
     switch (mode) {
         case 0: return launch_one<D, BF, 0, WK>(p, g, st);
         case kCap: return launch_one<D, BF, kCap, WK>(p, g, st);
@@ -479,6 +486,10 @@ static hipError_t launch_mode(const AttnParams& p, dim3 g, hipStream_t st) {
         case kDocs | kCap: return launch_one<D, BF, kDocs | kCap, WK>(p, g, st);
         case kDocs | kBias: return launch_one<D, BF, kDocs | kBias, WK>(p, g, st);
         case kDocs | kCap | kBias: return launch_one<D, BF, kDocs | kCap | kBias, WK>(p, g, st);
+        case kClose | kCap: return launch_one<D, BF, kClose | kCap, WK>(p, g, st);
+        case kClose | kCap | kBias: return launch_one<D, BF, kClose | kCap | kBias, WK>(p, g, st);
+        case kClose | kDocs | kCap: return launch_one<D, BF, kClose | kDocs | kCap, WK>(p, g, st);
+        case kClose | kDocs | kCap | kBias: return launch_one<D, BF, kClose | kDocs | kCap | kBias, WK>(p, g, st);
         case kSplit: return launch_one<D, BF, kSplit, WK>(p, g, st);
         case kSplit | kCap: return launch_one<D, BF, kSplit | kCap, WK>(p, g, st);
         default: return hipErrorInvalidValue;   // parts have neither documents nor a bias

@@ -189,15 +189,16 @@ __device__ __forceinline__ float half_sum(float x) {
     return __uint_as_float(s[0]) + __uint_as_float(s[1]);
 }
 
-// cap * tanh(y).  tanh as (1 - e) / (1 + e) with e = exp(-2 |y|), below 0.25,
-// where 1 - e would cancel, as its series to y^9 (next term under 1e-8 of y):
-// within about 2e-7 of the value, so a score of 12 is off by 2e-6.
-__device__ __forceinline__ float capped(float y, float cap) {
-    const float a = fabsf(y), y2 = y * y;
+// The score scale * s capped: cap tanh(y), y = yscale * s, yscale = scale / cap.  tanh as
+// (1 - e) / (1 + e) with e = exp(-2 |y|); below |y| = 0.25, where 1 - e would cancel,
+// x = scale * s times its series in y^2 (next term under 1e-8): within 16 * 2^-24 of the
+// value whatever the cap is, up to those of which y and cap are at the ends of fp32.
+__device__ __forceinline__ float capped(float s, float yscale, float scale, float cap) {
+    const float y = s * yscale, x = s * scale, a = fabsf(y), y2 = y * y;
     const float e = __builtin_amdgcn_exp2f(-2.0f * kLog2e * a);
-    const float big = (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e);
-    const float small = a + a * y2 * (-1.0f / 3 + y2 * (2.0f / 15 + y2 * (-17.0f / 315 + y2 * (62.0f / 2835))));
-    return cap * copysignf(a < 0.25f ? small : big, y);
+    const float big = cap * (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e);
+    const float small = x + x * y2 * (-1.0f / 3 + y2 * (2.0f / 15 + y2 * (-17.0f / 315 + y2 * (62.0f / 2835))));
+    return a < 0.25f ? small : copysignf(big, x);
 }
 
 // ---- non-finite values in masked places ----
