@@ -11,7 +11,9 @@
  * nothing synchronises, validation before any launch), and:
  *   - Elements are SLTX_F16 or SLTX_BF16, of one type in a call.  Scores, softmax
  *     statistics and sums are fp32; softmax weights are rounded to the element
- *     type before they meet v, the output once more.
+ *     type before they meet v, the output once more.  An fp16 weight keeps its 11
+ *     binary digits down to 2^-22 of the row's largest, and counts as nothing below
+ *     2^-33 of it.
  *   - head_dim is a multiple of 8, at most 128.  q_heads is a multiple of
  *     kv_heads; query head h reads key/value head h / (q_heads / kv_heads).
  *   - Strides are in elements, of dimensions batch, row and head; head_dim is

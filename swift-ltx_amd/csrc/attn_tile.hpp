@@ -262,16 +262,18 @@ __device__ __forceinline__ void weigh_values(f32x16 (&o)[D / 32], const u32x4 (&
 // ---- running softmax of one lane's column ----
 // Weights are exp2(f x - mf), with x the (capped, biased) score.  mf is f times
 // the largest score at some time past, plus kSpare: the row's largest weight
-// then is 2^-kSpare, and as long as no score is kSpare + 1 above it in the
-// exponent, every weight is below 2 and nothing has to be rescaled.  So the
-// weights are formed without a look at the maximum, and one or of their bits
-// tells afterwards whether one reached 2 (or is an infinity or NaN): the top bit
-// of the exponent.  Only then is the maximum taken, and the step done again
-// (grow).  bf16 has range to spare; fp16 keeps 11 binary digits of weights down
-// to 2^-11 of the largest, and 2^-22 of it below.
+// then is 2^-kSpare, and as long as the 16 weights of a lane sum to less than kMost,
+// nothing has to be rescaled.  So the weights are formed without a look at the maximum,
+// and their sum tells afterwards whether one may have left that range (or is an
+// infinity or NaN).  Only then is the maximum taken, and the step done again (grow).
+// bf16 has fp32's range: any scale serves.  fp16 does not: its largest weight
+// is 2^8 or more, 2^15 less at most, so that it keeps 11 binary digits of weights down to
+// 2^-22 of the largest, and loses those below 2^-33 of it, more than 2^22 of which it
+// would take to add up to the output's last digit.  After grow 16 weights sum to 2^-3
+// (bf16) or 2^12 (fp16) at most: no row grows twice for one maximum.
 template <bool BF>
 struct RowState {
-    static constexpr float kSpare = BF ? 7.0f : 3.0f;
+    static constexpr float kSpare = BF ? 7.0f : -8.0f, kMost = BF ? 2.0f : 32768.0f;
     // Nothing seen so far: finite, so that masked scores (-inf) get the weight 0
     // and any other an infinite one.
     static constexpr float kNone = -3.4028235e38f;
@@ -279,9 +281,9 @@ struct RowState {
 
     // p = weights of 32 keys as P^T fragments, rounded to nearest; sum = their sum
     // as rounded, so that the output is a mean of values, or unrounded where it
-    // will divide fp32 weights (EXACT).  Returns whether a weight of this lane is 2
-    // or more.  BIASED: a bias may be as low as the type goes, where
-    // f x overflows, so the difference is taken first.
+    // will divide fp32 weights (EXACT).  Returns whether the lane's weights have left
+    // their range.  BIASED: a bias may be as low as the type goes, where f x overflows,
+    // so the difference is taken first.
     template <bool BIASED, bool EXACT>
     __device__ __forceinline__ bool weigh(const f32x16& x, float f, u32x4 (&p)[2], float& sum) const {
         float a = 0.0f, b = 0.0f;
@@ -296,10 +298,7 @@ struct RowState {
             else i % 4 ? b = add2<BF>(w, b) : a = add2<BF>(w, a);
         }
         sum = a + b;
-        uint32_t bits = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) bits |= p[i / 4][i % 4];
-        return (bits & 0x40004000u) != 0;
+        return !(sum < kMost);
     }
 
     // Keys of a block of 32: their weights, with grow where a lane needs it.
@@ -312,7 +311,7 @@ struct RowState {
     }
 
     // The same with the maximum taken first, and what was summed so far rescaled,
-    // in the lanes of rows with such a weight: no row's result depends on others.
+    // in the lanes of such rows: no row's result depends on others.
     template <bool BIASED, bool EXACT, int DB>
     __device__ __forceinline__ void grow(bool mine, const f32x16& x, float f, u32x4 (&p)[2], float& sum,
                                          f32x16 (&o)[DB]) {
