@@ -306,6 +306,8 @@ def kv_accept(cache, drafted, path=None, count=None, stream=None):
             raise ValueError("path is an int32 [batch, n] tensor")
         n = int(path.shape[1])
         path = _need(path, "path", (cache.batch, n), (torch.int32,), cache.device).data_ptr()
+        # an empty tensor has no address, and no address means no path: another's stands for it
+        path = path or cache.length.data_ptr()
     count = _opt(count, "count", (cache.batch,), torch.int32, cache.device)
     with _launch(cache.k, stream) as handle:
         _P.check(_P.lib().sltx_kv_accept(cache._ref, drafted, path, n, count, handle))
