@@ -91,8 +91,10 @@ def _halves():
     return (torch.float16, torch.bfloat16)
 
 
-def _opt(t, what, shape, dtype, device):
-    return None if t is None else _need(t, what, shape, (dtype,), device).data_ptr()
+def _opt(t, what, shape, dtype, device, empty=None):
+    """The address of a tensor, or None.  One of no elements has no address; `empty`
+    stands for it where no address would mean no tensor."""
+    return None if t is None else _need(t, what, shape, (dtype,), device).data_ptr() or empty
 
 
 def attention(q, k, v, scale, *, softcap=0.0, bias=None, bias_zero=0, causal=False, prefix=None,
@@ -137,7 +139,7 @@ def attention(q, k, v, scale, *, softcap=0.0, bias=None, bias_zero=0, causal=Fal
     i32 = torch.int32
     a.prefix = _opt(prefix, "prefix", (B,), i32, dev)
     a.q_docs = _opt(q_docs, "q_docs", (B, Sq), i32, dev)
-    a.k_docs = _opt(k_docs, "k_docs", (B, Sk), i32, dev)
+    a.k_docs = _opt(k_docs, "k_docs", (B, Sk), i32, dev, empty=q.data_ptr())   # of no keys
     a.q_lens = _opt(q_lens, "q_lens", (B,), i32, dev)
     a.k_lens = _opt(k_lens, "k_lens", (B,), i32, dev)
     with _launch(q, stream) as handle:
@@ -305,9 +307,7 @@ def kv_accept(cache, drafted, path=None, count=None, stream=None):
         if path.dim() != 2:
             raise ValueError("path is an int32 [batch, n] tensor")
         n = int(path.shape[1])
-        path = _need(path, "path", (cache.batch, n), (torch.int32,), cache.device).data_ptr()
-        # an empty tensor has no address, and no address means no path: another's stands for it
-        path = path or cache.length.data_ptr()
+        path = _opt(path, "path", (cache.batch, n), torch.int32, cache.device, empty=cache.length.data_ptr())
     count = _opt(count, "count", (cache.batch,), torch.int32, cache.device)
     with _launch(cache.k, stream) as handle:
         _P.check(_P.lib().sltx_kv_accept(cache._ref, drafted, path, n, count, handle))

@@ -28,3 +28,20 @@ def test_accept_of_an_empty_path(pkg, dev):
         pkg.kv_accept(cache, 5, path=path[:1])
     with pytest.raises(pkg.SltxError, match="drafted"):
         pkg.kv_accept(cache, -1, path=path)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_documents_of_no_keys(pkg, dev, causal):
+    """No keys, with documents: every row sees nothing."""
+    import torch
+    q = torch.randn(2, 5, 4, 64, device=dev).half()
+    k = torch.zeros(2, 0, 2, 64, dtype=torch.float16, device=dev)
+    q_docs = torch.zeros(2, 5, dtype=torch.int32, device=dev)
+    k_docs = torch.zeros(2, 0, dtype=torch.int32, device=dev)
+    out = torch.full_like(q, 3.0)
+    assert pkg.attention(q, k, k, 0.1, q_docs=q_docs, k_docs=k_docs, causal=causal, out=out) is out
+    assert (out == 0).all()
+    with pytest.raises(pkg.SltxError, match="go together"):
+        pkg.attention(q, k, k, 0.1, k_docs=k_docs)
+    with pytest.raises(pkg.SltxError, match="go together"):
+        pkg.attention(q, k, k, 0.1, q_docs=q_docs)
