@@ -131,8 +131,8 @@ def attention(q, k, v, scale, *, softcap=0.0, bias=None, bias_zero=0, causal=Fal
                          q_heads=Hq, kv_heads=Hk, head_dim=D, causal=1 if causal else 0, scale=scale,
                          softcap=softcap)
     if bias is not None:
-        if bias.dim() != 2 or bias.shape[0] not in (1, Hq):
-            raise ValueError(f"bias has shape {tuple(bias.shape)}, expected [{Hq} or 1, distances]")
+        if bias.dim() != 2 or bias.shape[0] not in (1, Hq) or bias.shape[1] == 0:
+            raise ValueError(f"bias has shape {tuple(bias.shape)}, expected [{Hq} or 1, distances (at least one)]")
         _need(bias, "bias", bias.shape, (torch.float32,), dev)
         a.bias, a.bias_len, a.bias_zero = bias.data_ptr(), bias.shape[1], bias_zero
         a.bias_head_stride = 0 if bias.shape[0] == 1 else bias.shape[1]

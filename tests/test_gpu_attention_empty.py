@@ -45,3 +45,11 @@ def test_documents_of_no_keys(pkg, dev, causal):
         pkg.attention(q, k, k, 0.1, k_docs=k_docs)
     with pytest.raises(pkg.SltxError, match="go together"):
         pkg.attention(q, k, k, 0.1, q_docs=q_docs)
+
+
+@pytest.mark.parametrize("heads", [1, 4])
+def test_bias_of_no_distances(pkg, dev, heads):
+    import torch
+    q = torch.randn(1, 5, 4, 64, device=dev).half()
+    with pytest.raises(ValueError, match="bias"):
+        pkg.attention(q, q, q, 0.1, bias=torch.zeros(heads, 0, device=dev))
