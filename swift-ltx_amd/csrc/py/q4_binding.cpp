@@ -42,7 +42,7 @@ SLTX_ENTRIES(X)
 
 PyObject* g_check = nullptr;        // __init__.check: raises for a status
 PyTypeObject* g_weight = nullptr;   // Q4Weight
-PyObject *s_weight, *s_scales, *s_biases, *s_K, *s_group_size, *s_cuda_stream;
+PyObject *s_weight, *s_scales, *s_biases, *s_K, *s_group_size, *s_cuda_stream, *s_device_index;
 
 // Not the plain accepted call: the Python code takes it from here.
 struct Decline {};
@@ -524,6 +524,7 @@ void* stream_on(PyObject* o, int device, bool allocates) {
     const c10::hip::HIPStream cur = c10::hip::getCurrentHIPStream();
     need(cur.device_index() == device);
     if (o == Py_None) return cur.stream();
+    if (!PyLong_CheckExact(o)) need(attr_i32(o, s_device_index) == device);
     void* st = stream(o);
     need(!allocates || st == cur.stream());
     return st;
@@ -723,5 +724,6 @@ PyMODINIT_FUNC PyInit__q4_binding(void) {
     s_K = PyUnicode_InternFromString("K");
     s_group_size = PyUnicode_InternFromString("group_size");
     s_cuda_stream = PyUnicode_InternFromString("cuda_stream");
+    s_device_index = PyUnicode_InternFromString("device_index");
     return PyModule_Create(&module);
 }
