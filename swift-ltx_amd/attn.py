@@ -334,7 +334,8 @@ class CachedAttention:
 
     config: a ModelConfig (heads, head_dim, rope_theta, rope_scaling).  A cache that
     tracks weights gets those of each decoded token and of a prompt's last 64.
-    softcap: the cap of the scores (0: none).  sinks, recent: as in kv_evict."""
+    softcap: the cap of the scores (0: none).  sinks, recent: as in kv_evict.  A
+    budget is below the cache's capacity."""
 
     WINDOW = 64    # tokens of a prompt whose attention weights count
 
@@ -346,8 +347,14 @@ class CachedAttention:
                              f"{cache.layers}, {cache.batch}, {cache.kv_heads}, {cache.head_dim}")
         if cache.dtype != _halves()[0]:
             raise ValueError(f"the projections are fp16, the cache {cache.dtype}")
-        if budget is not None and cache.weight is None:
-            raise ValueError("a budget needs a cache that tracks weights")
+        if budget is not None:
+            if cache.weight is None:
+                raise ValueError("a budget needs a cache that tracks weights")
+            if not 0 < budget < cache.capacity:
+                raise ValueError(f"a budget of {budget} entries in a capacity of {cache.capacity}, which needs room for "
+                                 "the next token beside them")
+            if sinks < 0 or recent < 0 or sinks + recent > budget:
+                raise ValueError(f"{sinks} first and {recent} recent positions in a budget of {budget}")
         self.cache, self.stream, self.softcap = cache, stream, float(softcap)
         self.heads, self.kv_heads, self.head_dim = c.num_attention_heads, c.num_key_value_heads, c.head_dim
         self.scale = 1.0 / math.sqrt(c.head_dim)
