@@ -70,6 +70,8 @@ class PrefillStep:
                     raise ValueError(f"layer {i}: {name} is not a 4-bit weight")
         if (cache is None and options) or (cache is not None and attention is not None):
             raise ValueError("either an attention, or a cache and its options")
+        if cache is not None and self.S > cache.capacity:
+            raise ValueError(f"a prompt of {self.S} tokens for a cache with a capacity of {cache.capacity}")
         self.cached = None if cache is None else CachedAttention(c, cache, stream, **options)
         self.attention = self.cached or attention or q_columns_attention(self.q_dim)
         dev = weights.embed_tokens.weight.device

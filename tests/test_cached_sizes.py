@@ -36,3 +36,13 @@ def test_good_budgets(pkg):
     for options in (dict(), dict(budget=99), dict(budget=36), dict(budget=50, sinks=20, recent=30),
                     dict(budget=1, sinks=0, recent=0)):
         pkg.CachedAttention(_config(), _cache(), **options)
+
+
+def test_prompt_longer_than_the_cache(pkg):
+    """Refused before its buffers are made: the last rows would not see their own keys."""
+    from swiftltx_amd.prefill import PrefillStep
+    torch = pytest.importorskip("torch")
+    weights = SimpleNamespace(config=_config(), layers=[], embed_tokens=SimpleNamespace(weight=torch.zeros(1)))
+    for n in (101, 5000):
+        with pytest.raises(ValueError, match="capacity"):
+            PrefillStep(weights, n, cache=_cache())
