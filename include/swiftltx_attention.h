@@ -123,7 +123,8 @@ int64_t sltx_attention_cached_workspace(const sltx_kv_cache* cache, int32_t toke
  * of which the first count[b] (NULL: all) count.  In every layer and head, slot
  * length[b] + i takes the entry of slot length[b] + path[b, i]; then length and
  * next_position grow by the number accepted.  A path ends before an index outside
- * [0, drafted) and before a token that the capacity had no room for.  path NULL:
+ * [0, drafted), before a token that the capacity had no room for, and at the
+ * capacity, which it can reach by naming a token more than once.  path NULL:
  * the first count[b] (NULL: all) tokens as they stand. */
 int sltx_kv_accept(const sltx_kv_cache* cache, int32_t drafted, const int32_t* path, int32_t path_len,
                    const int32_t* count, void* stream);

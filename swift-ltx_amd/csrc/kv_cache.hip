@@ -193,15 +193,16 @@ hipError_t launch_kv_append(const AppendParams& p, hipStream_t st) {
 constexpr int kMaxPath = 64;
 
 // The tokens of sequence b's path that are accepted: its first count[b], as far
-// as they name drafted tokens that are in the cache.  One wave; all lanes.
+// as they name drafted tokens that are in the cache, and have a slot themselves (a path
+// that names a token twice may be longer than the room is).  One wave; all lanes.
 __device__ __forceinline__ int accepted(const CacheParams& c, int b, int drafted, const int32_t* path,
                                         int path_len, const int32_t* count, int* node) {
     const int lane = threadIdx.x & 63;
     const int most = count ? min(max(count[b], 0), path_len) : path_len;
     const int length = c.length[b];
     *node = lane < path_len ? path ? path[(int64_t)b * path_len + lane] : lane : -1;
-    const bool good = lane < most && *node >= 0 && *node < drafted && (int64_t)length + *node < c.capacity &&
-                      length >= 0;
+    const bool good = lane < most && *node >= 0 && *node < drafted && length >= 0 &&
+                      (int64_t)length + max(*node, lane) < c.capacity;
     const uint64_t bad = ~__ballot(good);
     return bad ? __builtin_ctzll(bad) : 64;
 }
