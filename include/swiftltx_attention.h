@@ -96,7 +96,8 @@ typedef struct sltx_kv_cache {
  * length[b] + t, with weight 0 and the token's position.  Pairs of values are
  * (i, i + pairs), or with `interleaved` (2i, 2i + 1); values past 2 * pairs pass
  * unchanged (pairs may be 0, with inv_freq NULL).  Tokens past the capacity are
- * dropped.  The sequence's length stays: every layer appends at the same place. */
+ * dropped.  The sequence's length stays: every layer appends at the same place.
+ * The cache's k and v must not overlap. */
 int sltx_kv_append(const void* q, const int64_t q_stride[3], const void* k, const int64_t k_stride[3],
                    const void* v, const int64_t v_stride[3], const sltx_kv_cache* cache, int32_t layer,
                    int32_t tokens, int32_t q_heads, const float* inv_freq, int32_t pairs,

@@ -373,6 +373,7 @@ int sltx_kv_append(const void* q, const int64_t q_stride[3], const void* k, cons
         if (overlap(t, tk) || overlap(t, tv)) return set_error(kErrInvalid, "%s: %s overlaps the cache", fn, t.name);
     }
     if (overlap(to, tk) || overlap(to, tv)) return set_error(kErrInvalid, "%s: q_out overlaps the cache", fn);
+    if (overlap(tk, tv)) return set_error(kErrInvalid, "%s: k and v of the cache overlap", fn);
     if (!aligned(depth, 4)) return set_error(kErrInvalid, "%s: misaligned depth", fn);
     if ((rc = require_device()) != kOk) return rc;
     AppendParams p{};
