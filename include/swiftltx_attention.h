@@ -20,6 +20,11 @@
  *     contiguous.  Strides of inputs are multiples of 8, may be 0 (broadcast)
  *     and may interleave (columns of one q|k|v projection); data pointers are
  *     16-byte aligned; 64 rows of k or v span less than 2 GB.
+ *   - Up to 2^28 rows or keys of a sequence (rows: tokens times the query heads of a
+ *     key/value head, over a cache), 2^28 slots of a cache, 65535 query heads in
+ *     sltx_attention and 65535 layers x sequences x heads of a cache; row strides of k and v below
+ *     2^24.  More is SLTX_ERR_UNSUPPORTED.  A call of more than 2^23 blocks (of at least
+ *     64 rows of a head, or one appended token) is refused by its launch.
  *   - A row that sees no key gives zeros.  A key that a row does not see does
  *     not touch it, whatever it holds (infinities and NaN included); a NaN that
  *     a row does see gives NaN.

@@ -296,8 +296,8 @@ def kv_append(q, k, v, cache, layer, inv_freq=None, *, depth=None, interleaved=F
 def kv_accept(cache, drafted, path=None, count=None, stream=None):
     """Of `drafted` tokens appended in every layer, those of `path` (int32 [batch, n],
     n <= 64: indices among the drafted, root first), the first count[b] of them
-    (int32 [batch]; None: all), become the sequences' next entries; without a path
-    the first count[b] (None: all) drafted tokens."""
+    (int32 [batch]; None: all), become the sequences' next entries, up to the
+    capacity; without a path the first count[b] (None: all) drafted tokens."""
     native = _native()
     if native is not None and native.kv_accept(*cache._handle, drafted, path, count, stream):
         return

@@ -13,7 +13,8 @@
 // TB/s; eight sequences of 3000 26 us, 3.8 TB/s.  The kernel of many rows, made to take
 // the same calls, has fewer waves at work on few keys: 12.8 us instead of 11.2 for 4000
 // keys (head_dim 64: 10.6 instead of 9.6), but is up to a tenth faster at head_dim 128
-// over many (eight sequences of 3000 23.9 us).
+// over many (eight sequences of 3000 23.9 us).  Which of the two it is goes by the
+// lengths, which are on the device: calls of at most 32 rows take this one.
 #include "attn_tile.hpp"
 
 namespace sltx {

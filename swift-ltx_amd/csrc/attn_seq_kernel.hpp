@@ -9,11 +9,12 @@
 // One pass over the keys with a running maximum and sum; nothing but the output
 // is written.
 //
-// 4 head_dim products a score on the matrix units and about 9 vector instructions,
-// one of them an exponential; the two overlap in part only.  At head_dim 64 the
-// scores cost as much as the products: 6144 rows and keys of 32 heads, bf16, 340 to
-// 357 us, 871 to 908 TFLOP/s, where a large product reaches 1190 to 1245 (the clock
-// falls with the power that either draws).  Head_dim 128 halves the scores: 8192
+// 4 head_dim operations a score on the matrix units and about 4 vector instructions,
+// one of them an exponential at a quarter of the others' rate.  At head_dim 64 the
+// scores cost more than the products: 6144 rows and keys of 32 heads, bf16, 340 to
+// 382 us, 810 to 908 TFLOP/s, where a large product reaches 1190 to 1245.  Counters
+// (about 1.9 GHz): the matrix units are busy in 40% of a SIMD's cycles, vector
+// instructions are at work in 53%.  Head_dim 128 halves the scores: 8192
 // causal rows of 32 heads, two sequences, 1057 to 1096 us, 1003 to 1040 TFLOP/s;
 // 4096 rows of one 152 us, 900.  A tile takes 1.0 us for 64 rows and 64 keys of
 // head_dim 128, mostly the chain of its steps, so that few rows (750 behind 1300
